@@ -340,30 +340,46 @@ def _plain_write(state, case, t):
 
 
 def _plain_attn(state, case, t):
-    nkv, rep, hd, block = case["nkv"], case["rep"], case["hd"], case["block"]
-    scale = 1.0 / math.sqrt(hd)
-    at = 0
-    for b, (past, new) in enumerate(zip(*state["lengths"])):
-        if new == 0:
-            continue
-        n = past + new
-        pages = t["tables"][b, :_ceil(n, block)].long()
-        pos = torch.arange(past, n, device="cuda")[:, None]
-        key = torch.arange(n, device="cuda")[None, :]
-        hidden = key > pos
-        if case["window"]:
-            hidden = hidden | (key <= pos - case["window"])
-        for h in range(nkv) if new * n > 1 << 20 else (slice(0, nkv),):
-            heads = slice(h, h + 1) if isinstance(h, int) else h
-            k = t["k_cache"][pages, heads].transpose(0, 1).reshape(-1, pages.numel() * block, hd)[:, :n].float()
-            v = t["v_cache"][pages, heads].transpose(0, 1).reshape(-1, pages.numel() * block, hd)[:, :n].float()
-            q = t["q"][at:at + new].view(new, nkv, rep, hd)[:, heads].permute(1, 2, 0, 3).float()
-            s = (q.reshape(q.shape[0], rep * new, hd) @ k.transpose(1, 2).contiguous() * scale).view(-1, rep, new, n)
-            s = s.masked_fill_(hidden, -math.inf)
-            w = torch.exp(s - s.amax(-1, keepdim=True))
-            o = (w.view(-1, rep * new, n) @ v).view(-1, rep, new, hd) / w.sum(-1, keepdim=True)
-            t["o"][at:at + new].view(new, nkv, rep, hd)[:, heads] = o.permute(2, 0, 1, 3).to(t["o"].dtype)
-        at += new
+    """Requests with about as many rows go together, padded to the largest of them."""
+    nkv, rep = case["nkv"], case["rep"]
+    past, new = state["lengths"]
+    starts = _prefix(new)
+    groups = {}
+    for b, n in enumerate(new):
+        if n:
+            groups.setdefault(n.bit_length(), []).append(b)
+    for bs in groups.values():
+        rows, keys = max(new[b] for b in bs), max(past[b] + new[b] for b in bs)
+        # as many requests at a time as leave the scores at 2 GiB, and a long prompt by its key heads
+        some = max(1, (1 << 29) // (nkv * rep * rows * keys))
+        heads = 1 if nkv * rep * rows * keys > 1 << 29 else nkv
+        for i in range(0, len(bs), some):
+            for h in range(0, nkv, heads):
+                _plain_group(case, t, [(past[b], new[b], starts[b], b) for b in bs[i:i + some]], slice(h, h + heads))
+
+
+def _plain_group(case, t, reqs, heads):
+    rep, hd, block = case["rep"], case["hd"], case["block"]
+    past, new, start, b = (torch.tensor(x).cuda() for x in zip(*reqs))
+    rows, keys = max(r[1] for r in reqs), max(r[0] + r[1] for r in reqs)
+    pages = t["tables"][b, :_ceil(keys, block)].clamp(min=0).long()
+    k, v = (t[n][:, heads][pages].transpose(1, 2).reshape(len(reqs), -1, pages.shape[1] * block, hd)[:, :, :keys].float()
+            for n in ("k_cache", "v_cache"))
+    i = torch.arange(rows, device="cuda")
+    live = i < new[:, None]
+    at = (start[:, None] + i).clamp(max=t["q"].shape[0] - 1)
+    nkv = k.shape[1]
+    q = t["q"].view(t["q"].shape[0], case["nkv"], rep, hd)[at][:, :, heads].permute(0, 2, 3, 1, 4).reshape(len(reqs), nkv, rep * rows, hd).float()
+    s = (q @ k.transpose(2, 3).contiguous() * (1.0 / math.sqrt(hd))).view(len(reqs), nkv, rep, rows, keys)
+    pos, key = (past[:, None] + i)[:, None, None, :, None], torch.arange(keys, device="cuda")
+    hidden = key > pos
+    if case["window"]:
+        hidden = hidden | (key <= pos - case["window"])
+    s.masked_fill_(hidden, -math.inf)
+    w = torch.exp_(s.sub_(s.amax(-1, keepdim=True)))
+    o = (w.view(len(reqs), nkv, rep * rows, keys) @ v).view(s.shape[:4] + (hd,)) / w.sum(-1, keepdim=True)
+    o = o.permute(0, 3, 1, 2, 4)[live].to(t["o"].dtype)
+    t["o"].view(t["o"].shape[0], case["nkv"], rep, hd)[at[live], heads] = o
 
 
 def _plain_verify(state, case, t):

@@ -181,8 +181,53 @@ typedef struct sanic_sched {
     int32_t variant;
 } sanic_sched;
 
-/* Stage kinds (/root/reference/src/partition.rs:44-98). */
-enum { SANIC_STAGE_FUSED = 0, SANIC_STAGE_POINTWISE = 1 };
+/* Stage kinds (/root/reference/src/partition.rs:44-98). OPERATOR has no counterpart there: a stage
+ * whose result is no fold and no elementwise value of its inputs, because it indexes by whole
+ * numbers that other stages computed, ends where the data says, or has several results. It is named
+ * by `op` and takes its operands as leaves (below). */
+enum { SANIC_STAGE_FUSED = 0, SANIC_STAGE_POINTWISE = 1, SANIC_STAGE_OPERATOR = 2 };
+
+/* Operators over a ragged batch and a paged cache. A batch of B requests is token-major: request b
+ * brings the rows starts[b] <= r < starts[b + 1] of a step's T rows, behind the past[b] tokens that
+ * its cache holds, so row r stands at position past[b] + r - starts[b]. Rows from starts[B] on
+ * belong to no request: what an operator writes by row is left as it was there. The cache is a pool
+ * of NB blocks of BS tokens, [NB, NKV, BS, HD] for keys and for values; block tables[b][i] holds
+ * request b's positions i·BS to i·BS + BS - 1. Counts, lengths, blocks and slots are U32 buffers;
+ * SANIC_NONE stands for no block, slot or token, and every index is checked on the device: a block
+ * or slot past the pool is none, a start past T is T.
+ *
+ * BLOCK_TABLES  leaves past [B], new [B], held [B + 1], free [F], tables [B, M] (STATE, in place),
+ *               slots [T], positions [T], held_next [B + 1]; output starts [B + 1]; stream = BS.
+ *               starts = the exclusive prefix sum of new, cut at T. held[b] blocks stand in
+ *               tables[b], held[B] blocks are taken from `free`; a request with rows takes as many
+ *               more, in the order of the requests, as its past + new positions need, as the table's
+ *               M entries and the list's F blocks allow. Only the new entries of `tables` are
+ *               written. slots[r] = block · BS + position mod BS, or SANIC_NONE without a block.
+ *               B at most 8192.
+ * CACHE_WRITE   leaves k [T, NKV, HD], v [T, NKV, HD], slots [T], starts [B + 1], the key cache and
+ *               the value cache (STATE, in place); output the key cache. Row r goes to slot slots[r]
+ *               in the cache's type; slots of one step differ from each other.
+ * PAGED_ATTN    leaves q [T, NH, HD], key cache, value cache, tables [B, M], starts [B + 1],
+ *               past [B], scale (CONST); output [T, NH, HD]; stream = window, 0 = none. Query head h
+ *               reads key head h / (NH / NKV). A row at position p sees the keys of positions
+ *               j <= p, with a window j > p - window; keys without a block are not seen. Softmax of
+ *               scale·q·k over them, in f32, times the values; a row that sees nothing is 0.
+ * VERIFY_DRAFTS leaves p [T, V], q [T, V] (or -1), tokens [T], u [T], draw [B], starts [B + 1],
+ *               accepted [B]; output tokens [T]. tokens[r + 1] is the draft behind row r of the same
+ *               request; p[r] are the target's probabilities there, q[r] those it was drawn from (no
+ *               q: it was certain). Drafts are accepted in order while u[r]·q < p; behind the last
+ *               accepted one a token is drawn: from max(p - q, 0) at a refused draft, from p behind
+ *               the last draft or where nothing is left, the lowest index whose running sum exceeds
+ *               draw[b] times the sum (sums in f64). Output: the accepted drafts, the drawn token,
+ *               then SANIC_NONE; accepted[b] = the number of drafts accepted.
+ *
+ * The float operands (q, k, v, the caches) may be affine views of their buffers. CACHE_WRITE and
+ * BLOCK_TABLES write what their inputs say whatever the state held before, so a program whose only
+ * in-place stages are operators runs under sanic_hip_execute_static too. A buffer that a stage
+ * writes may not overlap another buffer of that stage (SANIC_ERR_ARG), and operand buffers start at
+ * addresses that are multiples of 4. */
+enum { SANIC_OPR_BLOCK_TABLES = 1, SANIC_OPR_CACHE_WRITE, SANIC_OPR_PAGED_ATTN, SANIC_OPR_VERIFY_DRAFTS };
+#define SANIC_NONE 0xFFFFFFFFu
 
 /* Leaf axis binding: leaf dim -> a grid dim (>= 0), the streamed axis, or broadcast. */
 #define SANIC_BIND_STREAM (-1)
@@ -199,6 +244,7 @@ typedef struct sanic_stage {
     int32_t n_leaves;
     int32_t leaf[SANIC_MAX_LEAVES];                  /* node index                        */
     int32_t bind[SANIC_MAX_LEAVES][SANIC_MAX_RANK];  /* per leaf dim                      */
+    int32_t op;                  /* OPERATOR: which one (SANIC_OPR_*); its operands are leaf[] */
     sanic_carrier carrier;
     int32_t epilogue;            /* node tree over FOLD (+ other inputs), -1 = none       */
     sanic_sched sched;
@@ -304,7 +350,8 @@ int sanic_hip_execute(sanic_hip_exe* exe, sanic_hip_buffer* const* bindings, int
  * each waits for the previous eager call's work on that GPU, whichever device handle (stream)
  * made it. A call made while the device's stream is being captured into a HIP graph is not
  * ordered that way: replays of such a graph that overlap other calls on the GPU race on the
- * scratch. In-place programs are refused as by sanic_hip_execute. */
+ * scratch. In-place programs are refused as by sanic_hip_execute, but for those whose in-place stages
+ * are operators: these write what their inputs say whatever the state held. */
 int sanic_hip_execute_static(sanic_hip_exe* exe, sanic_hip_buffer* const* bindings, int n_bindings);
 
 /* No counterpart in the reference. The number of device allocations (hipMalloc) this library

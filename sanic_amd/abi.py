@@ -41,7 +41,7 @@ SCHED_DT = np.dtype([("lane_stream", "<i4"), ("waves", "<i4"), ("chunk", "<i4"),
 STAGE_DT = np.dtype([
     ("kind", "<i4"), ("out_buffer", "<i4"), ("out_dtype", "<i4"), ("rank", "<i4"),
     ("grid", "<i8", MAX_RANK), ("stream", "<i8"), ("n_leaves", "<i4"),
-    ("leaf", "<i4", MAX_LEAVES), ("bind", "<i4", (MAX_LEAVES, MAX_RANK)),
+    ("leaf", "<i4", MAX_LEAVES), ("bind", "<i4", (MAX_LEAVES, MAX_RANK)), ("op", "<i4"),
     ("carrier", CARRIER_DT), ("epilogue", "<i4"), ("sched", SCHED_DT), ("value", "<i4"),
     ("where", "<i4"),
 ], align=True)

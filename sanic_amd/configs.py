@@ -73,7 +73,8 @@ def precompile_all() -> None:
     for s in (None, Sched(lane_stream=True, waves=1), Sched(lane_stream=True, waves=2, split=4)):
         direct_attention(sched=s).precompile()
     for p in (rmsnorm_projection(kmajor=False), rmsnorm_projection(kmajor=True), int4_matmul(),
-              decode_attention(), llama_decode(), flash_prefill(), flash_prefill(window=1024)):
+              decode_attention(), llama_decode(), flash_prefill(), flash_prefill(window=1024),
+              paged_step(), draft_verification()):
         p.precompile()
     # every tiling variant the measured tuner may try (each stage takes variant v when it has
     # more than v; identical sources compile once)
@@ -278,4 +279,44 @@ def decode_attention(NH: int = 32, NKV: int = 8, HD: int = 64, cap: int = 4096,
     vexp = ir.permute(ir.expand_heads(vc, 0, rep), (0, 2, 1))
     p.fused("o", (NH, HD), cap, [(scores, (0, STREAM)), (vexp, (0, STREAM, 1))],
             C.online_softmax_weighted(), out_dtype, sched=sched)
+    return p
+
+
+def paged_step(T: int = 64, B: int = 8, NH: int = 32, NKV: int = 8, HD: int = 64, NB: int = 2048, BS: int = 16, M: int = 256,
+               theta: float = 500000.0, window: int = 0, dtype: int = ir.BF16) -> Program:
+    """The attention of one serving step over a ragged batch of up to B requests and T new rows: a
+    request's rows may be a prompt, a chunk of one, one decoded token, or a token with its drafts.
+    Block tables and slots come from the lengths, q and k are rotated at each row's position, k and v
+    go into the paged caches (states, block ids from the list `free` of NB) and every row attends to
+    its request's keys. q, k and v are token-major, as a projection of [T, hidden] leaves them
+    (q [T, NH·HD]). `plan.held` is the next step's `held`."""
+    p = Program()
+    p.state("tables", (B, M), ir.U32)
+    kc, vc = (p.state(n, (NB, NKV, BS, HD), dtype) for n in ("k_cache", "v_cache"))
+    past, new = p.input("past", (B,), ir.U32), p.input("new", (B,), ir.U32)
+    plan = p.block_tables("plan", past, new, p.input("held", (B + 1,), ir.U32), p.input("free", (NB,), ir.U32), "tables", block=BS, rows=T)
+    invf = ir.rope_inv_freq(theta, HD // 2)
+
+    def rotated(name, heads):
+        x = ir.permute(ir.split(p.input(name, (T, heads * HD), dtype), 1, heads, HD), (1, 0, 2))     # [heads, T, HD]
+        return p.pointwise(f"{name}.rope", ir.permute(ir.rope(x, plan.positions, invf), (1, 0, 2)), dtype, role=3)
+
+    q, k = rotated("q", NH), rotated("k", NKV)
+    v = ir.split(p.input("v", (T, NKV * HD), dtype), 1, NKV, HD)
+    p.cache_write("write", k, v, plan.slots, plan.starts, kc, vc)
+    p.paged_attention("o", q, kc, vc, plan.tables, plan.starts, past, window=window, out_dtype=dtype)
+    return p
+
+
+def draft_verification(T: int = 40, B: int = 8, V: int = 128256, temperature: float = 1.0) -> Program:
+    """Drafts against the target's logits [T, V]: softmax(logits / temperature) in f32, its
+    maximum and normaliser folds over the vocabulary, then the acceptance and the drawn token."""
+    p = Program()
+    z = ir.map_(ir.MUL, p.input("logits", (T, V), ir.F32), ir.const(1.0 / temperature))
+    top = p.fused("top", (T,), V, [(z, (0, STREAM))], C.plain(ir.M_MAX), ir.F32, role=3)
+    e = ir.map_(ir.EXP, ir.map_(ir.SUB, z, ir.unsqueeze(top, 1)))
+    mass = p.fused("mass", (T,), V, [(e, (0, STREAM))], C.plain(ir.M_ADD), ir.F32, role=3)
+    probs = p.pointwise("probs", ir.map_(ir.DIV, e, ir.unsqueeze(mass, 1)), ir.F32, role=3)
+    p.verify_drafts("check", probs, p.input("draft_probs", (T, V), ir.F32), p.input("tokens", (T,), ir.U32), p.input("starts", (B + 1,), ir.U32),
+                    p.input("u", (T,), ir.F32), p.input("draw", (B,), ir.F32))
     return p

@@ -15,6 +15,7 @@
 // All arithmetic is f32 (accumulators included); loads widen from the storage dtype and the
 // single store narrows through it (emit_metal.rs:162-232).
 #include "emit.h"
+#include "operators.h"
 #include "skeletons.h"
 
 #include <algorithm>
@@ -285,6 +286,8 @@ void validate(const sanic_program_desc* d) {
             if (vn.rank > st.rank) bad("value rank");
             if (tree_has_fold(d, st.value)) bad("pointwise value reads a fold");
             if (st.where >= 0 && st.where >= d->n_nodes) bad("where node");
+        } else if (st.kind == SANIC_STAGE_OPERATOR) {
+            validate_operator(d, s);
         } else {
             bad("unknown stage kind");
         }
@@ -1543,6 +1546,7 @@ LoweredStage lower_pointwise(const sanic_program_desc* d, int si) {
 // float, bf16 and nibble formats; such stages take the generic renderer.
 static bool stage_touches_q8(const sanic_program_desc* d, int s) {
     const sanic_stage& st = d->stages[s];
+    if (st.kind == SANIC_STAGE_OPERATOR) return false;
     if (d->buffers[st.out_buffer].dtype == SANIC_Q8) return true;
     std::vector<int> todo;
     if (st.kind == SANIC_STAGE_FUSED) {
@@ -1568,6 +1572,11 @@ static Lowered lower_stages(const sanic_program_desc* d) {
     t_counter_bytes = 0;
     for (int s = 0; s < d->n_stages;) {
         const sanic_stage& st = d->stages[s];
+        if (st.kind == SANIC_STAGE_OPERATOR) {
+            out.stages.push_back(lower_operator(d, s, out.scratch_bytes));
+            s++;
+            continue;
+        }
         // skeletons may batch or absorb the next few stages: none of them may touch Q8 either
         bool generic = getenv("SANIC_HIP_GENERIC") != nullptr;
         for (int t = s; t < std::min(d->n_stages, s + 8) && !generic; t++) generic = stage_touches_q8(d, t);

@@ -16,6 +16,7 @@
 #include <thread>
 
 #include "emit.h"
+#include "operators.h"
 
 namespace sanic {
 
@@ -123,6 +124,9 @@ struct sanic_hip_exe {
     std::vector<sanic_buffer_desc> buffers;
     std::vector<int> stage_out;       // output buffer of each stage
     std::vector<int> stage_out_role;
+    bool operators_in_place = true;   // every stage that writes a state is an operator
+    // per operator stage: the buffers it writes, then those it only reads
+    std::vector<std::pair<std::vector<int>, std::vector<int>>> operands;
     Lowered low;
     std::map<std::string, std::shared_ptr<Module>> modules;  // source -> module
     ~sanic_hip_exe() {
@@ -190,7 +194,10 @@ __device__ void store_from_float(void* p, int dt, float scale, int64_t i, float 
 
 __global__ void sanic_convert(const void* src, int sdt, float sscale, void* dst, int ddt, float dscale, int64_t n) {
     int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < n) store_from_float(dst, ddt, dscale, i, load_as_float(src, sdt, sscale, i));
+    if (i >= n) return;
+    // whole numbers of 32 bits do not pass through a float's 24
+    if (sdt == SANIC_U32 && ddt == SANIC_U32) ((uint32_t*)dst)[i] = ((const uint32_t*)src)[i];
+    else store_from_float(dst, ddt, dscale, i, load_as_float(src, sdt, sscale, i));
 }
 
 // ── helpers ──────────────────────────────────────────────────────────────────────────────
@@ -310,6 +317,32 @@ static void check_binding(sanic_hip_exe* exe, int i, sanic_hip_buffer* b) {
         fail(SANIC_ERR_SHAPE, "program buffer " + std::to_string(i) + " binding holds " + std::to_string(b->bytes) +
                                   " bytes; its shape needs " + std::to_string(buffer_bytes(bd)));
     if (b->dev != exe->dev) fail(SANIC_ERR_ARG, "binding lives on another device");
+}
+
+// Operators index their buffers by what other buffers hold, so a result that overlaps another
+// operand of its stage would change what the launch still reads; their wide loads take any address
+// that is a multiple of 4.
+static void check_operands(const sanic_hip_exe* exe, char* const* at) {
+    for (auto& o : exe->operands) {
+        auto each = [&](int i, bool written) {
+            if ((uintptr_t)at[i] % 4) fail(SANIC_ERR_ARG, "program buffer " + std::to_string(i) + ": an operator's buffers start at multiples of 4 bytes");
+            if (written) return;
+            for (int w : o.first) {
+                const int64_t nw = buffer_bytes(exe->buffers[w]), ni = buffer_bytes(exe->buffers[i]);
+                if (i != w && at[i] < at[w] + nw && at[w] < at[i] + ni)
+                    fail(SANIC_ERR_ARG, "program buffers " + std::to_string(w) + " and " + std::to_string(i) + " overlap: an operator writes one of them");
+            }
+        };
+        for (size_t k = 0; k < o.first.size(); k++) {
+            each(o.first[k], true);
+            for (size_t l = 0; l < k; l++) {
+                const int x = o.first[k], y = o.first[l];
+                if (at[x] < at[y] + buffer_bytes(exe->buffers[y]) && at[y] < at[x] + buffer_bytes(exe->buffers[x]))
+                    fail(SANIC_ERR_ARG, "program buffers " + std::to_string(x) + " and " + std::to_string(y) + " overlap: an operator writes both");
+            }
+        }
+        for (int i : o.second) each(i, false);
+    }
 }
 
 // ── SANIC_DEBUG (the reference's debug levels, lib.rs:25-46, compile.rs:1141-1300) ─────────
@@ -528,6 +561,13 @@ int sanic_hip_prepare(sanic_hip_device* dev, const sanic_program_desc* desc, san
         for (int s = 0; s < desc->n_stages; s++) {
             exe->stage_out.push_back(desc->stages[s].out_buffer);
             exe->stage_out_role.push_back(desc->buffers[desc->stages[s].out_buffer].role);
+            if (desc->stages[s].kind == SANIC_STAGE_OPERATOR) {
+                exe->operands.push_back({operator_writes(desc, desc->stages[s]), operator_reads(desc, desc->stages[s])});
+                for (int b : exe->operands.back().first)
+                    if (desc->buffers[b].role == SANIC_BUF_STATE) exe->stage_out_role.back() = SANIC_BUF_STATE;
+            } else if (exe->stage_out_role.back() == SANIC_BUF_STATE) {
+                exe->operators_in_place = false;
+            }
         }
         compile_all(exe.get(), true);
         if (debug_level() >= 1) dump_schedule("schedule", desc, exe->low);
@@ -605,6 +645,7 @@ int sanic_hip_execute(sanic_hip_exe* exe, sanic_hip_buffer* const* bindings, int
         std::vector<std::unique_ptr<sanic_hip_buffer>> owned;
         std::unique_ptr<sanic_hip_buffer> scratch;
         bind_all(exe, bindings, n_bindings, bound, owned, scratch);
+        check_operands(exe, addresses(bound).data());
         enqueue(exe, addresses(bound).data(), scratch->ptr(), counters_of(exe, scratch.get()));
         SANIC_HIP(hipStreamSynchronize(exe->dev->stream));
         for (int i = 0; i < (int)exe->buffers.size(); i++) outputs[i] = nullptr;
@@ -619,7 +660,7 @@ int sanic_hip_execute_static(sanic_hip_exe* exe, sanic_hip_buffer* const* bindin
     return guarded([&] {
         if (!exe || !bindings) fail(SANIC_ERR_ARG, "null argument");
         for (int r : exe->stage_out_role)
-            if (r == SANIC_BUF_STATE)
+            if (r == SANIC_BUF_STATE && !exe->operators_in_place)
                 fail(SANIC_ERR_IN_PLACE, "this program writes state in place; use sanic_hip_capture");
         const int nb = (int)exe->buffers.size();
         if (n_bindings != nb) fail(SANIC_ERR_ARG, "expected " + std::to_string(nb) + " bindings, got " + std::to_string(n_bindings));
@@ -652,6 +693,7 @@ int sanic_hip_execute_static(sanic_hip_exe* exe, sanic_hip_buffer* const* bindin
         if (need > kStaticScratchBytes)
             fail(SANIC_ERR_ARG, "this program needs " + std::to_string(need) + " bytes of scratch; the static scratch holds " +
                                     std::to_string(kStaticScratchBytes));
+        check_operands(exe, at);
         SANIC_HIP(hipSetDevice(exe->dev->ordinal));
         hipStream_t s = exe->dev->stream;
         std::lock_guard<std::mutex> lk(g_static_mu);
@@ -734,6 +776,7 @@ int sanic_hip_capture(sanic_hip_exe* exe, sanic_hip_buffer* const* bindings, int
         auto rp = std::make_unique<sanic_hip_replay>();
         rp->exe = exe;
         bind_all(exe, bindings, n_bindings, rp->bound, rp->owned, rp->scratch);
+        check_operands(exe, addresses(rp->bound).data());
         int nb = (int)exe->buffers.size();
         for (int p = 0; p < n_pairs; p++) {
             int o = feedback[2 * p], i = feedback[2 * p + 1];

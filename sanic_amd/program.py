@@ -9,6 +9,8 @@ leaves are node trees over program buffers.
 from __future__ import annotations
 
 import ctypes
+import math
+from collections import namedtuple
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -19,6 +21,14 @@ from .carrier import Carrier, ExprTable
 
 INPUT, STATE, OUTPUT, SCRATCH = range(4)
 STREAM, BCAST = -1, -2
+
+# operators (include/sanic_hip.h SANIC_OPR_*) and the whole number that stands for no block, slot
+# or token
+BLOCK_TABLES, CACHE_WRITE, PAGED_ATTN, VERIFY_DRAFTS = 1, 2, 3, 4
+NONE = 0xFFFFFFFF
+
+BlockTables = namedtuple("BlockTables", "starts slots positions held tables")
+Verified = namedtuple("Verified", "tokens accepted")
 
 
 @dataclass
@@ -50,7 +60,7 @@ class BufferDecl:
 
 @dataclass
 class Stage:
-    kind: int                       # 0 fused, 1 pointwise
+    kind: int                       # 0 fused, 1 pointwise, 2 operator
     name: str
     out: BufferDecl
     grid: Tuple[int, ...]
@@ -61,6 +71,7 @@ class Stage:
     sched: Sched = field(default_factory=Sched)
     value: Optional[ir.Node] = None
     where: Optional[ir.Node] = None
+    op: int = 0                     # operator: which one
 
 
 class Program:
@@ -123,6 +134,78 @@ class Program:
         self.stages.append(Stage(1, name, out, grid, value=value, where=where))
         return self.node(out.name)
 
+    # ── operators over a ragged batch and a paged cache (include/sanic_hip.h SANIC_STAGE_OPERATOR) ──
+    def _operator(self, op: int, name: str, out: BufferDecl, operands, size: int = 0):
+        leaves = [(n, ()) for n in operands]
+        self.stages.append(Stage(2, name, out, tuple(out.shape), int(size), leaves, op=op))
+
+    def _operand(self, x) -> ir.Node:
+        return self.node(x) if isinstance(x, str) else x
+
+    def block_tables(self, name: str, past, new, held, free, tables, block: int, rows: int, role: int = OUTPUT) -> BlockTables:
+        """Where a step's new tokens go, from the requests' lengths. Request b holds `past[b]`
+        tokens and brings `new[b]` (u32 [B]); `held` (u32 [B + 1]) counts the blocks that stand in
+        each line of the state `tables` (u32 [B, M]) and, last, those taken from the list `free`
+        (u32 [F]). Each request, in order, gets the blocks of `block` tokens that its new positions
+        need, while the table's line and the list last; only those entries of `tables` are written.
+
+        Declares `<name>.starts` [B + 1] (request b has the rows from starts[b] to starts[b + 1]; cut
+        at `rows`), `<name>.slots` and `<name>.positions` [rows] (slot = block·block size + offset,
+        NONE where no block is left; rows behind the last request are left as they were) and
+        `<name>.held` [B + 1], `held` for the next step. Calling it again with the same inputs
+        writes the same results. A request whose tokens were taken back (rejected drafts) keeps its
+        blocks: `past` may fall, `held` stays."""
+        past, new, held, free, tables = (self._operand(x) for x in (past, new, held, free, tables))
+        B = past.shape[0]
+        starts = self._decl(f"{name}.starts", role, (B + 1,), ir.U32)
+        slots = self._decl(f"{name}.slots", role, (rows,), ir.U32)
+        positions = self._decl(f"{name}.positions", role, (rows,), ir.U32)
+        after = self._decl(f"{name}.held", role, (B + 1,), ir.U32)
+        self._operator(BLOCK_TABLES, name, starts,
+                       [past, new, held, free, tables, self.node(slots.name), self.node(positions.name), self.node(after.name)], block)
+        return BlockTables(*(self.node(b.name) for b in (starts, slots, positions, after)), tables)
+
+    def cache_write(self, name: str, k, v, slots, starts, k_cache, v_cache):
+        """Write the step's rows k and v [T, NKV, HD] into the paged caches (states
+        [NB, NKV, BS, HD], or a view of one with these dims) at their slots, converted to the cache's
+        type with one rounding. Rows behind the last request and slots past the pool (NONE among
+        them) write nothing; slots of one step differ from each other. Returns the cache nodes."""
+        k, v, slots, starts, kc, vc = (self._operand(x) for x in (k, v, slots, starts, k_cache, v_cache))
+        src = kc
+        while src.inputs:
+            src = src.inputs[0]
+        self._operator(CACHE_WRITE, name, self.by_name[src.name], [k, v, slots, starts, kc, vc])
+        return kc, vc
+
+    def paged_attention(self, name: str, q, k_cache, v_cache, tables, starts, past, scale: Optional[float] = None,
+                        window: int = 0, out_dtype=ir.BF16, role: int = OUTPUT) -> ir.Node:
+        """Causal attention of a step's rows q [T, NH, HD] over the paged caches
+        [NB, NKV, BS, HD], which hold the step's own rows too: request b's row i stands at
+        past[b] + i and sees the keys up to there, with `window` > 0 the last `window` of them. Query
+        head h reads key head h // (NH // NKV). A row that sees no key is 0; rows behind the last
+        request are left as they were. `scale` defaults to 1/√HD."""
+        q, kc, vc, tables, starts, past = (self._operand(x) for x in (q, k_cache, v_cache, tables, starts, past))
+        out = self._decl(name, role, q.shape, out_dtype)
+        scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+        self._operator(PAGED_ATTN, name, out, [q, kc, vc, tables, starts, past, ir.const(scale)], window)
+        return self.node(name)
+
+    def verify_drafts(self, name: str, p, q, tokens, starts, u, draw, role: int = OUTPUT) -> Verified:
+        """Accept or refuse drafted tokens so that what comes out is distributed as the target's own
+        samples. tokens[r + 1] (u32 [T]) is the draft behind row r of the same request, p [T, V] the
+        target's probabilities at each row and q [T, V] those the draft was drawn from (None: it was
+        certain, as from a lookup). Drafts are accepted in order while u[r]·q < p (u f32 [T], uniform
+        in [0, 1)); then one more token is drawn by draw[b] (f32 [B], uniform in [0, 1)): from
+        max(p − q, 0) where a draft was refused, from p behind the last one.
+
+        Declares `<name>.tokens` [T] (a request's accepted drafts, the drawn token, then NONE; rows
+        behind the last request are left as they were) and `<name>.accepted` [B]."""
+        p, tokens, starts, u, draw = (self._operand(x) for x in (p, tokens, starts, u, draw))
+        out = self._decl(f"{name}.tokens", role, tokens.shape, ir.U32)
+        accepted = self._decl(f"{name}.accepted", role, draw.shape, ir.U32)
+        self._operator(VERIFY_DRAFTS, name, out, [p, None if q is None else self._operand(q), tokens, u, draw, starts, self.node(accepted.name)])
+        return Verified(self.node(out.name), self.node(accepted.name))
+
     def repeat_stage(self, i: int, copies: int, fresh_inputs: bool = False) -> List[str]:
         """Append `copies` more instances of stage `i`, each writing its own output buffer
         (for timing one kernel as back-to-back launches inside one captured graph). With
@@ -130,6 +213,8 @@ class Program:
         (`<name>.copy<r>`), so back-to-back launches do not find each other's inputs in cache."""
         import copy as _copy
         st = self.stages[i]
+        if st.kind == 2 and st.op != PAGED_ATTN:
+            raise ValueError("an operator with several results is not repeated")
         names = []
         for r in range(copies):
             name = f"{st.out.name}.copy{r}"
@@ -157,7 +242,7 @@ class Program:
                         m = n
                     memo[id(n)] = m
                     return m
-                if st.kind == 0:
+                if st.kind in (0, 2):
                     dup.leaves = [(ren(nd), b) for nd, b in st.leaves]
                     dup.epilogue = ren(st.epilogue) if st.epilogue is not None else None
                 else:
@@ -183,7 +268,13 @@ class Program:
             r["epilogue"] = -1
             r["value"] = -1
             r["where"] = -1
-            if s.kind == 0:
+            if s.kind == 2:
+                r["op"] = s.op
+                r["stream"] = s.stream
+                r["n_leaves"] = len(s.leaves)
+                r["leaf"] = [-1 if n is None else nt.add(n) for n, _ in s.leaves] + [-1] * (abi.MAX_LEAVES - len(s.leaves))
+                r["bind"] = -3
+            elif s.kind == 0:
                 r["stream"] = s.stream
                 r["n_leaves"] = len(s.leaves)
                 leaf = [-1] * abi.MAX_LEAVES

@@ -76,6 +76,10 @@ void emit_point_fold(Renderer& R, Code& code, const sanic_stage& st, const std::
 // `n` arrival counters of the program being lowered on this thread: their byte offset from the
 // program's first (a kernel argument Arg::COUNTERS).
 int64_t take_counters(int64_t n);
+// Scratch and arrival counters of operator stages: the stages of a program run one after the other and
+// leave their counters at zero, so they share one area of each (the largest any of them asks for).
+int64_t shared_scratch(int64_t& scratch, int64_t bytes);
+int64_t shared_counters(int64_t n);
 // Bytes of the static scratch of sanic_hip_execute_static. A program whose first lowering needs more
 // is lowered again without the kernels that a form with less scratch can stand in for (lean).
 const int64_t kStaticScratchBytes = int64_t(32) << 20;

@@ -60,6 +60,24 @@ int64_t take_counters(int64_t n) {
     return at;
 }
 
+// [offset, size) of what the operator stages of the program being lowered share
+static thread_local int64_t t_shared_scratch[2], t_shared_counters[2];
+int64_t shared_scratch(int64_t& scratch, int64_t bytes) {
+    if (bytes > t_shared_scratch[1]) {
+        t_shared_scratch[0] = scratch;
+        t_shared_scratch[1] = (bytes + 255) / 256 * 256;
+        scratch += t_shared_scratch[1];
+    }
+    return t_shared_scratch[0];
+}
+int64_t shared_counters(int64_t n) {
+    if (n > t_shared_counters[1]) {
+        t_shared_counters[0] = take_counters(n);
+        t_shared_counters[1] = n;
+    }
+    return t_shared_counters[0];
+}
+
 void emit_arrival(Code& k, const std::string& flag, const std::string& tid, const std::string& cnt,
                   const std::string& expected, bool xcd_local) {
     k.line("__shared__ int " + flag + ";");
@@ -1570,6 +1588,7 @@ static bool stage_touches_q8(const sanic_program_desc* d, int s) {
 static Lowered lower_stages(const sanic_program_desc* d) {
     Lowered out;
     t_counter_bytes = 0;
+    for (int64_t* shared : {t_shared_scratch, t_shared_counters}) shared[0] = shared[1] = 0;
     for (int s = 0; s < d->n_stages;) {
         const sanic_stage& st = d->stages[s];
         if (st.kind == SANIC_STAGE_OPERATOR) {

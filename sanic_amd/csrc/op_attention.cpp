@@ -79,27 +79,818 @@ extern "C" __global__ void __launch_bounds__(256) sanic_paged_attn(Args a) {
 }
 )SRC";
 
+// The matrix-core kernel: bf16 or f16 queries and caches, heads of a multiple of 16 up to 256.
+//
+// A workgroup (4 waves) takes one key head's rows of one request: the NH / NKV query heads that read
+// it and the request's new rows are one axis (packed row = row · REP + head), since they share every
+// key. Few rows (up to DR = 32, a decoded token or its drafts): the four waves split a tile's keys in
+// groups of 16 (and, with tiles of 32 keys, the value dims) and meet in LDS at the end. More rows: a
+// workgroup takes PR = 128 of them, 32 a wave, and each wave goes over all keys. Either way tiles of
+// TK keys come straight from the pages into a ring of LDS buffers (16 bytes a lane, no register
+// staging), addressed through the item's part of the block table in LDS.
+//
+// Work is split over keys too: request lengths are known on the device alone, so every workgroup sums
+// the requests' key tiles and derives the same split length, such that the items fill the chip a few
+// times over and their partials fit the scratch; it then finds its own item in the prefix sums. The
+// parts of one row meet in the workgroup that arrives last, which adds them in split order.
+//
+// Scores are computed transposed (Sᵀ = K·Qᵀ), so a lane owns one row's column: softmax statistics are
+// lane-local plus two lane swaps, and Sᵀ's layout is the B operand of Oᵀ = Vᵀ·P as it stands. Softmax
+// runs in base 2, t = s·(scale·log2 e); the reference moves only when a tile's maximum exceeds it by
+// 8, so weights reach 2^8 and rescaling is rare; sums come from the matrix cores (ones times P), of the
+// weights as rounded for the product.
+static const char* kMfma = R"SRC(
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef sanic_elem<DO>::T o_t;
+struct Args { const unsigned short *q, *k, *v; const unsigned *tables, *starts, *past; o_t* o; float* part; unsigned* counts; };
+
+constexpr bool HALF = DQ == 2;
+constexpr int CH = HD / 8;                       // 16-byte chunks of a key's row
+constexpr int DSTEP = (HD + 31) / 32;            // products over 32 head dims, the last one's upper half 0 if HD is odd times 16
+constexpr int DT = HD / 16;
+constexpr int LOADS = (TK * CH + 255) / 256;     // 16-byte loads a lane for a tile's keys, and its values
+constexpr int TILE = LOADS * 256 * 8;            // elements of a staged tile, the last lanes' surplus included
+constexpr int KG = TK / 16, DH = 4 / KG, DTH = (DT + DH - 1) / DH;
+constexpr int MBS = M * BS;                      // positions a block table can hold
+constexpr float NEG_INF = -__builtin_huge_valf();
+
+__device__ __forceinline__ f32x4 mma32(s16x8 x, s16x8 y, f32x4 c) {
+  if constexpr (HALF) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, x), __builtin_bit_cast(b16x8, y), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(s16x4 x, s16x4 y, f32x4 c) {
+  if constexpr (HALF) return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, x), __builtin_bit_cast(f16x4, y), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(x, y, c, 0, 0, 0);
+}
+// four values rounded to the matrix cores' type (ties to even), and what the rounding left
+__device__ __forceinline__ u32x2 pack(f32x4& x) {
+  u32x2 out;
+  #pragma unroll
+  for (int e = 0; e < 2; e++) {
+    if constexpr (HALF) {
+      const f16x2 h = {(_Float16)x[2 * e], (_Float16)x[2 * e + 1]};
+      x[2 * e] -= (float)h[0], x[2 * e + 1] -= (float)h[1];
+      out[e] = __builtin_bit_cast(unsigned, h);
+    } else {
+      const unsigned h = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){x[2 * e], x[2 * e + 1]}, b16x2));
+      x[2 * e] -= __uint_as_float(h << 16), x[2 * e + 1] -= __uint_as_float(h & 0xFFFF0000u);
+      out[e] = h;
+    }
+  }
+  return out;
+}
+__device__ __forceinline__ float quad_max(float v) {  // over the 4 lanes of a row's column
+  return sanic_rows_max(v);
+}
+// a chunk's place in its row of the staged tile: rotated by the row, so that the 16 rows a wave reads
+// at one dim lie in different banks
+__device__ __forceinline__ int spot(int row, int c) {
+  if constexpr ((CH & (CH - 1)) == 0 && CH >= 4) return c ^ (row & (CH < 16 ? CH - 1 : 15));
+  else return (c + row) % CH;
+}
+__device__ __forceinline__ int chunk_at(int row, int at) {  // its inverse
+  if constexpr ((CH & (CH - 1)) == 0 && CH >= 4) return at ^ (row & (CH < 16 ? CH - 1 : 15));
+  else return (at + CH - row % CH) % CH;
+}
+__device__ __forceinline__ int clamp_pos(long long p) { return p < 0 ? 0 : p > MBS ? MBS : (int)p; }
+
+// (one object: with several, the compiler waits for every load into LDS before any read of it)
+__shared__ struct {
+  __attribute__((aligned(16))) unsigned short ring[STAGES][2][TILE];
+  unsigned pages[PAGES];
+  unsigned long long odd_keys;
+  int holes, last_arrival;
+} lds;
+
+// ── what this workgroup does ──────────────────────────────────────────────────────────────────────
+struct Item {
+  int b, tile, split, splits, rows, slot, count;
+  long long start, past;
+};
+struct Req {
+  long long start, past;
+  int rows, tiles, kt;
+};
+__device__ __forceinline__ Req request(const Args& a, int b) {
+  Req q{0, 0, 0, 0, 0};
+  if (b >= B) return q;
+  const long long s = a.starts[b] < T ? a.starts[b] : T, e = a.starts[b + 1] < T ? a.starts[b + 1] : T;
+  if (e <= s) return q;
+  q.start = s, q.past = a.past[b];
+  q.rows = (int)(e - s) * REP;
+  q.tiles = q.rows <= DR ? 0 : (q.rows + PR - 1) / PR;
+  const int hi = clamp_pos(q.past + (e - s)), lo = W ? clamp_pos(q.past + 1 - W) : 0;
+  const int kt = (hi + TK - 1) / TK - lo / TK;
+  q.kt = kt > 1 ? kt : 1;
+  return q;
+}
+__device__ __forceinline__ int pick(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ long long pick(long long v, int lane) {
+  return (long long)((unsigned long long)(unsigned)pick((int)(v >> 32), lane) << 32 | (unsigned)pick((int)v, lane));
+}
+__device__ __forceinline__ int scan64(int v) {  // inclusive, over the wave
+  for (int o = 1; o < 64; o <<= 1) {
+    const int n = __shfl_up(v, o);
+    if ((threadIdx.x & 63) >= o) v += n;
+  }
+  return v;
+}
+// Every wave of every workgroup computes the same numbers in the same order. P: requests of more than
+// DR rows, D: the others.
+__device__ __forceinline__ bool find_item(const Args& a, int it, Item& o) {
+  const int lane = threadIdx.x & 63;
+  float ud = 0, rd = 0, urd = 0, up = 0, tp = 0;
+  int items = 0;
+  Req q;
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    q = request(a, b0 + lane);
+    const bool d = q.tiles == 0;
+    ud += d ? q.kt : 0, rd += d ? q.rows : 0, urd += d ? (float)q.rows * q.kt : 0;
+    up += (float)q.tiles * q.kt, tp += q.tiles;
+  }
+  ud = sanic_wave_sum(ud), rd = sanic_wave_sum(rd), urd = sanic_wave_sum(urd);
+  if (PITEMS) up = sanic_wave_sum(up), tp = sanic_wave_sum(tp);
+  // split lengths in key tiles: items = Σ ⌈kt / length⌉ ≤ Σ kt / length + requests
+  const float never = 1e9f;
+  float ld = ud / DTARGET, lp = never;
+  const float room = (float)DROWS - rd - 1.0f;
+  if (room < rd) ld = never;
+  else ld = __builtin_fmaxf(ld, urd / room);
+  if (PITEMS && 2.0f * tp <= (float)PSPLIT) lp = up / ((float)PSPLIT - tp - 1.0f);
+  // (the sums are f32: 1.001 covers their roundings where a bound hangs on them)
+  const int len_d = __builtin_amdgcn_readfirstlane((int)__builtin_fmaxf(1.0f, __builtin_ceilf(__builtin_fminf(ld * 1.001f, never))));
+  const int len_p = __builtin_amdgcn_readfirstlane((int)__builtin_fmaxf(1.0f, __builtin_ceilf(__builtin_fminf(lp * 1.001f, never))));
+  // the many-row items first: they take longest
+  if (PITEMS) {
+    int before_t = 0;
+    for (int b0 = 0; b0 < B; b0 += 64) {
+      if (B > 64) q = request(a, b0 + lane);
+      int splits = (q.kt + len_p - 1) / len_p;
+      if (splits > MEET / PR) splits = MEET / PR;
+      const int mine = q.tiles * splits, inc = scan64(mine), tinc = scan64(q.tiles);
+      const unsigned long long who = __ballot(mine > 0 && it >= inc - mine && it < inc);
+      if (who) {
+        const int l = __builtin_ctzll(who), x = it - pick(inc - mine, l), tiles = pick(q.tiles, l);
+        o.b = b0 + l, o.splits = pick(splits, l), o.rows = pick(q.rows, l);
+        o.tile = tiles - 1 - x / o.splits;     // the last rows see most
+        o.split = x % o.splits;
+        o.slot = (int)DROWS + (items + it - o.split) * (int)PR;
+        o.count = (int)B + before_t + pick(tinc, l) - tiles + o.tile;
+        o.start = pick(q.start, l), o.past = pick(q.past, l);
+        return true;
+      }
+      const int all = pick(inc, 63);
+      it -= all, items += all, before_t += pick(tinc, 63);
+    }
+  }
+  int before_r = 0;
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    if (B > 64) q = request(a, b0 + lane);
+    int splits = (q.kt + len_d - 1) / len_d;
+    if (q.rows && splits > MEET / q.rows) splits = MEET / q.rows;
+    const int mine = q.tiles == 0 && q.rows ? splits : 0, inc = scan64(mine), rinc = scan64(mine * q.rows);
+    const unsigned long long who = __ballot(mine > 0 && it >= inc - mine && it < inc);
+    if (who) {
+      const int l = __builtin_ctzll(who);
+      o.b = b0 + l, o.tile = -1, o.splits = pick(mine, l), o.rows = pick(q.rows, l);
+      o.split = it - pick(inc - mine, l);
+      o.slot = before_r + pick(rinc - mine * q.rows, l);
+      o.count = o.b;
+      o.start = pick(q.start, l), o.past = pick(q.past, l);
+      return true;
+    }
+    it -= pick(inc, 63), before_r += pick(rinc, 63);
+  }
+  return false;
+}
+
+// ── tiles of keys and values ──────────────────────────────────────────────────────────────────────
+struct Stream {
+  const Args& a;
+  const unsigned* table;
+  int g, first_page, last_page, base;   // the pages seen by any row; the first page in LDS
+  const unsigned short *k, *v;
+
+  // the block table from page p on into LDS (every thread, between two barriers)
+  __device__ __forceinline__ void pages_from(int p) {
+    base = p;
+    bool hole = false;
+    for (int i = threadIdx.x; i < PAGES; i += 256) {
+      const int at = p + i;
+      unsigned x = at <= last_page ? table[at] : 0xFFFFFFFFu;
+      hole |= x >= NB && at >= first_page && at <= last_page;
+      lds.pages[i] = x;
+    }
+    if (hole) lds.holes = 1;
+  }
+  __device__ __forceinline__ bool covers(int t0) const { return t0 / BS >= base && (t0 + TK - 1) / BS < base + PAGES; }
+  __device__ __forceinline__ void fetch(int t0, int buf) const {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    #pragma unroll
+    for (int u = 0; u < LOADS; u++) {
+      const int i = (u * 4 + wave) * 64 + lane;
+      int row = i / CH;
+      const int c = chunk_at(row, i % CH) * 8;
+      if (TK * CH % 256 && row >= TK) row = TK - 1;
+      const int key = t0 + row;
+      const unsigned page = lds.pages[key / BS - base];
+      const long long pg = page < NB ? page : 0, in = key % BS;    // a page that is none is read as block 0 and masked
+      const unsigned short* kp = k + (pg * K0 + in * K2 + c);
+      const unsigned short* vp = v + (pg * V0 + in * V2 + c);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)kp, (__attribute__((address_space(3))) void*)&lds.ring[buf][0][(u * 4 + wave) * 512], 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vp, (__attribute__((address_space(3))) void*)&lds.ring[buf][1][(u * 4 + wave) * 512], 16, 0, 0);
+    }
+  }
+  // the key is in the pool (asked where a tile has keys that are not)
+  __device__ __forceinline__ bool there(int key) const {
+    const int p = key / BS;
+    return p >= first_page && p <= last_page && table[p] < NB;
+  }
+};
+
+// The first tiles under way. The query rows are waited for before them (behind the block table, which
+// is anyway): the compiler would otherwise wait for them, and so for every tile, inside the loop.
+template <int RT>
+__device__ __forceinline__ void begin(Stream& st, int t_first, int t_last, s16x8 (&q)[RT][DSTEP]) {
+  if (threadIdx.x == 0) lds.holes = 0;
+  __syncthreads();
+  if (t_first < t_last) st.pages_from(t_first * TK / (int)BS);
+  #pragma unroll
+  for (int t = 0; t < RT; t++)
+    #pragma unroll
+    for (int d = 0; d < DSTEP; d++) asm volatile("" : "+v"(q[t][d]));
+  __syncthreads();
+  if (t_first < t_last) st.fetch(t_first * TK, 0);
+  if (STAGES == 3 && t_first + 1 < t_last) {
+    if (!st.covers((t_first + 1) * TK)) {
+      __syncthreads();
+      st.pages_from((t_first + 1) * TK / (int)BS);
+      __syncthreads();
+    }
+    st.fetch((t_first + 1) * TK, 1);
+  }
+}
+// tile `i` of the item has arrived in every wave's part; PD tiles are under way behind it
+__device__ __forceinline__ void arrived(int left) {
+  constexpr int PD = STAGES - 1;
+  if (PD == 2 && left > 0) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+__device__ __forceinline__ s16x8 key_run(int buf, int row, int step, int lq) {
+  const int c = step * 4 + lq;
+  if (HD % 32 == 0 || c < CH) return *(const s16x8*)&lds.ring[buf][0][row * HD + spot(row, c) * 8];
+  return (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
+}
+// LDS address of a lane's part of a transposed read of 16 keys (from row `row0`) × 16 value dims
+__device__ __forceinline__ unsigned value_at(int buf, int row0, int dt, int l16, int lq) {
+  const int row = row0 + lq * 4 + (l16 >> 2), col = dt * 16 + (l16 & 3) * 4;
+  return (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned short*)&lds.ring[buf][1][row * HD + spot(row, col >> 3) * 8 + (col & 7)];
+}
+// Transposed reads (a lane gets 4 keys of one value dim), waited for in the same statement: the
+// compiler takes an asm output as written at once.
+__device__ __forceinline__ void tr_read4(unsigned a0, unsigned a1, unsigned a2, unsigned a3, s16x4& r0, s16x4& r1, s16x4& r2, s16x4& r3) {
+  asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %2, %6\n\tds_read_b64_tr_b16 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3) : "v"(a0), "v"(a1), "v"(a2), "v"(a3) : "memory");
+}
+__device__ __forceinline__ void tr_read1(unsigned a0, s16x4& r0) {
+  asm volatile("ds_read_b64_tr_b16 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(r0) : "v"(a0) : "memory");
+}
+__device__ __forceinline__ bool odd_value(unsigned short x) { return HALF ? (x & 0x7C00) == 0x7C00 : (x & 0x7F80) == 0x7F80; }
+
+// One column of scores into weights: s holds the products of keys key0 + 16·kt + r of row [lo, hi) and
+// leaves as 2^(t − m). `factor` is what the row's earlier sums are scaled by.
+template <int N>
+__device__ __forceinline__ void weigh(const Stream& st, f32x4 (&s)[N], bool full, bool any_hole, int key0, int lo, int hi, float& m, float& factor) {
+  float top = NEG_INF;
+  if (full) {
+    #pragma unroll
+    for (int kt = 0; kt < N; kt++) top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(top, s[kt][0]), __builtin_fmaxf(s[kt][1], s[kt][2])), s[kt][3]);
+    top *= C2;
+  } else {
+    #pragma unroll
+    for (int kt = 0; kt < N; kt++)
+      #pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int key = key0 + kt * 16 + r;
+        bool seen = key >= lo && key < hi;
+        if (any_hole && seen) seen = st.there(key);
+        s[kt][r] = seen ? s[kt][r] * C2 : NEG_INF;
+        top = __builtin_fmaxf(top, s[kt][r]);
+      }
+  }
+  factor = 1.0f;
+  if (!__all(top <= m + 8.0f && m > NEG_INF)) {
+    top = quad_max(top);
+    const float to = top > m + 8.0f ? top : m;
+    factor = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+    m = to;
+  }
+  // nothing seen so far, or scores of −inf alone: their weights are 0, 2^(−inf − 0)
+  const float ref = m == NEG_INF ? 0.0f : m;
+  #pragma unroll
+  for (int kt = 0; kt < N; kt++)
+    #pragma unroll
+    for (int r = 0; r < 4; r++) s[kt][r] = __builtin_amdgcn_exp2f(full ? __builtin_fmaf(s[kt][r], C2, -ref) : s[kt][r] - ref);
+}
+
+// Values that nobody in the workgroup sees become 0 (0·NaN would reach every row of the product);
+// where one that is seen is not finite, its key's bit is returned, and it is 0 in the tile: add_odd
+// adds it to the rows that see it. Rows [row0, row0 + rows) × chunks [c0, c0 + chunks), 64 lanes.
+__device__ __forceinline__ unsigned long long clean(const Stream& st, int buf, int t0, int row0, int rows, int c0, int chunks, int lo, int hi, int part, int parts) {
+  unsigned long long odd = 0;
+  for (int i = part; i < rows * chunks; i += parts) {
+    const int row = row0 + i / chunks, c = c0 + i % chunks, key = t0 + row;
+    s16x8* p = (s16x8*)&lds.ring[buf][1][row * HD + spot(row, c) * 8];
+    s16x8 x = *p;
+    bool dead = key < lo || key >= hi, change = false;
+    if (!dead && lds.holes) dead = !st.there(key);
+    #pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const bool o = odd_value((unsigned short)x[e]);
+      if (o && !dead) odd |= 1ull << row;
+      if (o || dead) x[e] = 0, change = true;
+    }
+    if (change) *p = x;
+  }
+  return odd;
+}
+template <int N, int D>
+__device__ __forceinline__ void add_odd(const Stream& st, unsigned long long odd, int t0, int rel, const f32x4 (&w)[N], f32x4 (&o)[D], int dt0, int lq) {
+  while (odd) {
+    const int row = __builtin_ctzll(odd), key = t0 + row;
+    odd &= odd - 1;
+    float x = 0.0f;
+    #pragma unroll
+    for (int kt = 0; kt < N; kt++)
+      #pragma unroll
+      for (int r = 0; r < 4; r++)
+        if (rel + kt * 16 + lq * 4 + r == row) x = w[kt][r];
+    x = sanic_rows_sum(x);
+    const unsigned page = st.table[key / BS];
+    if (page >= NB) continue;
+    const unsigned short* v = st.v + ((long long)page * V0 + key % BS * V2);
+    #pragma unroll
+    for (int d = 0; d < D; d++)
+      #pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int col = (dt0 + d) * 16 + lq * 4 + r;
+        if (col < HD && odd_value(v[col]) && x != 0.0f) o[d][r] += x * sanic_get<DQ>(__builtin_bit_cast(sanic_elem<DQ>::T, v[col]));
+      }
+  }
+}
+
+// ── the parts of a row ────────────────────────────────────────────────────────────────────────────
+// part: DROWS + PSPLIT·PR rows a key head, of HD sums and, behind all of those, the maximum and the sum
+__device__ __forceinline__ float* part_sums(const Args& a, int g, int slot) { return a.part + ((long long)g * SLOTS + slot) * HD; }
+__device__ __forceinline__ float* part_stats(const Args& a, int g, int slot) { return a.part + (long long)NKV * SLOTS * HD + ((long long)g * SLOTS + slot) * 2; }
+__device__ __forceinline__ long long out_at(const Item& it, int g, int row) {
+  return ((it.start + row / REP) * NH + g * REP + row % REP) * (long long)HD;
+}
+__device__ __forceinline__ void put4(o_t* p, f32x4 v) {
+  if constexpr (DO == 1) {
+    struct __attribute__((packed, aligned(4))) run { f32x4 v; };
+    ((run*)p)->v = v;
+  } else {
+    struct __attribute__((packed, aligned(4))) run { o_t e[4]; };
+    run x;
+    for (int e = 0; e < 4; e++) x.e[e] = sanic_put<DO>(v[e]);
+    *(run*)p = x;
+  }
+}
+// The splits of rows [row0, row0 + rows) meet: the last workgroup to arrive adds them in their order.
+// Split s of row r stands at slot + s·stride + r.
+__device__ __forceinline__ void meet(const Args& a, const Item& it, int g, int row0, int rows, int stride) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, splits = it.splits;
+  unsigned* cnt = a.counts + (long long)it.count * NKV + g;
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (tid == 0) {
+    lds.last_arrival = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)splits - 1u;
+    if (lds.last_arrival) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  }
+  __syncthreads();
+  if (!lds.last_arrival) return;
+  if (tid == 0) *cnt = 0;      // the next launch's arrivals count from 0 again
+  // weights of the splits, 2^(m − max m) / Σ (0 for a row that saw nothing): splits·rows ≤ MEET of them
+  float* w = (float*)lds.ring;
+  static_assert(MEET * 4 <= sizeof(lds.ring) && 4096 <= sizeof(lds.ring));
+  for (int r = wave; r < rows; r += 4) {
+    float mx = NEG_INF, sum = 0.0f;
+    for (int s = lane; s < splits; s += 64) mx = __builtin_fmaxf(mx, part_stats(a, g, it.slot + s * stride + r)[0]);
+    mx = sanic_wave_max(mx);
+    const float ref = mx == NEG_INF ? 0.0f : mx;
+    for (int s = lane; s < splits; s += 64) {
+      const float* p = part_stats(a, g, it.slot + s * stride + r);
+      const float f = __builtin_amdgcn_exp2f(p[0] - ref);
+      w[s * rows + r] = f;
+      sum += p[1] * f;
+    }
+    sum = sanic_wave_sum(sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    for (int s = lane; s < splits; s += 64) w[s * rows + r] *= inv;
+  }
+  __syncthreads();
+  // a thread's sums: 4 value dims of a row; with few of them, teams take every teams-th split each and
+  // meet in LDS
+  const int units = rows * (int)(HD / 4), teams = units >= 256 ? 1 : 256 / units;
+  if (teams == 1) {
+    for (int u = tid; u < units; u += 256) {
+      const int r = u / (int)(HD / 4), d = u % (int)(HD / 4) * 4;
+      f32x4 acc = {0, 0, 0, 0};
+      #pragma unroll 4
+      for (int s = 0; s < splits; s++) acc += w[s * rows + r] * *(const f32x4*)(part_sums(a, g, it.slot + s * stride + r) + d);
+      put4(a.o + out_at(it, g, row0 + r) + d, acc);
+    }
+    return;
+  }
+  const int team = tid / units, u = tid % units, r = u / (int)(HD / 4), d = u % (int)(HD / 4) * 4;
+  f32x4 acc = {0, 0, 0, 0};
+  if (team < teams) {
+    #pragma unroll 8
+    for (int s = team; s < splits; s += teams) acc += w[s * rows + r] * *(const f32x4*)(part_sums(a, g, it.slot + s * stride + r) + d);
+  }
+  __syncthreads();
+  f32x4* mine = (f32x4*)lds.ring;
+  mine[tid] = acc;
+  __syncthreads();
+  if (team == 0) {
+    for (int k = 1; k < teams; k++) acc += mine[k * units + tid];
+    put4(a.o + out_at(it, g, row0 + r) + d, acc);
+  }
+}
+
+// a lane's part of a query row; a negative scale is the query's
+__device__ __forceinline__ void read_row(const unsigned short* q, int lq, s16x8 (&x)[DSTEP]) {
+  struct __attribute__((packed, aligned(4))) run { s16x8 v; };
+  #pragma unroll
+  for (int s = 0; s < DSTEP; s++) {
+    x[s] = (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
+    if (HD % 32 == 0 || s * 4 + lq < CH) x[s] = ((const run*)(q + (s * 4 + lq) * 8))->v;
+    if (FLIP) x[s] ^= (short)0x8000;
+  }
+}
+
+// ── few rows: the waves split the tile's keys ─────────────────────────────────────────────────────
+template <int RT>
+__device__ __forceinline__ void few_rows(const Args& a, const Item& it, int g, Stream& st, int t_first, int t_last, int lo_all, int hi_all, int full_lo, int full_hi) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
+  const int kg = wave % KG, dh = wave / KG, dt0 = dh * DTH;
+  s16x8 qf[RT][DSTEP];
+  int lo[RT], hi[RT];
+  #pragma unroll
+  for (int t = 0; t < RT; t++) {
+    int row = t * 16 + l16;
+    if (row >= it.rows) row = it.rows - 1;
+    const unsigned short* q = a.q + (QB + (it.start + row / REP) * Q0 + (g * REP + row % REP) * Q1);
+    read_row(q, lq, qf[t]);
+    hi[t] = clamp_pos(it.past + row / REP + 1);
+    lo[t] = W ? clamp_pos(it.past + row / REP + 1 - W) : 0;
+  }
+  f32x4 o[RT][DTH], sum[RT];
+  float m[RT];
+  #pragma unroll
+  for (int t = 0; t < RT; t++) {
+    m[t] = NEG_INF, sum[t] = (f32x4){0, 0, 0, 0};
+    #pragma unroll
+    for (int d = 0; d < DTH; d++) o[t][d] = (f32x4){0, 0, 0, 0};
+  }
+  begin(st, t_first, t_last, qf);
+  const short one = HALF ? (short)0x3C00 : (short)0x3F80;
+  const s16x4 ones = {one, one, one, one};
+  int buf = 0;
+  for (int i = t_first; i < t_last; i++) {
+    const int t0 = i * TK;
+    arrived(t_last - 1 - i);
+    if (i + STAGES - 1 < t_last) {
+      const int ahead = t0 + (STAGES - 1) * TK;
+      if (!st.covers(ahead)) {
+        __syncthreads();
+        st.pages_from(ahead / BS);
+        __syncthreads();
+      }
+      st.fetch(ahead, buf == 0 ? STAGES - 1 : buf - 1);
+    }
+    const bool any_hole = lds.holes, full = t0 >= full_lo && t0 + TK <= full_hi && !any_hole;
+    unsigned long long odd = 0;
+    if (!full) {
+      const int c0 = dt0 * 2, c1 = (dt0 + DTH) * 2 < CH ? (dt0 + DTH) * 2 : CH;
+      odd = clean(st, buf, t0, kg * 16, 16, c0, c1 - c0, lo_all, hi_all, lane, 64);
+      for (int x = 1; x < 64; x <<= 1) odd |= __shfl_xor(odd, x);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    s16x4 vt[DTH];
+    #pragma unroll
+    for (int t = 0; t < RT; t++) {
+      f32x4 s[1] = {{0, 0, 0, 0}};
+      const int row = kg * 16 + l16;
+      #pragma unroll
+      for (int d = 0; d < DSTEP; d++) s[0] = mma32(key_run(buf, row, d, lq), qf[t][d], s[0]);
+      float factor;
+      weigh<1>(st, s, full, any_hole, t0 + kg * 16 + lq * 4, lo[t], hi[t], m[t], factor);
+      if (!__all(factor == 1.0f)) {
+        sum[t] *= factor;
+        #pragma unroll
+        for (int d = 0; d < DTH; d++) o[t][d] *= factor;
+      }
+      if (t == 0) {
+        #pragma unroll
+        for (int d = 0; d < DTH; d += 4) {
+          unsigned at[4];
+          #pragma unroll
+          for (int e = 0; e < 4; e++) at[e] = value_at(buf, kg * 16, dt0 + (d + e < DTH ? d + e : d) < DT ? dt0 + (d + e < DTH ? d + e : d) : 0, l16, lq);
+          if (d + 3 < DTH) tr_read4(at[0], at[1], at[2], at[3], vt[d], vt[d + 1], vt[d + 2], vt[d + 3]);
+          else {
+            #pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (d + e < DTH) tr_read1(at[e], vt[d + e]);
+          }
+        }
+      }
+      if (odd) add_odd<1, DTH>(st, odd, t0, kg * 16, s, o[t], dt0, lq);
+      #pragma unroll
+      for (int k = 0; k < FEW_TERMS; k++) {
+        const s16x4 p = __builtin_bit_cast(s16x4, pack(s[0]));
+        sum[t] = mma16(ones, p, sum[t]);
+        #pragma unroll
+        for (int d = 0; d < DTH; d++) o[t][d] = mma16(vt[d], p, o[t][d]);
+      }
+    }
+    buf = buf == STAGES - 1 ? 0 : buf + 1;
+  }
+  // the key groups meet: maxima and sums, then the outputs, group after group
+  __syncthreads();
+  float* stat = (float*)lds.pages;                       // [2][KG][16·RT], by the waves of the first dims
+  float* acc = (float*)lds.ring;                         // [KG][16·RT][HD]
+  if (dh == 0 && lq == 0) {
+    #pragma unroll
+    for (int t = 0; t < RT; t++) stat[kg * 32 + t * 16 + l16] = m[t], stat[128 + kg * 32 + t * 16 + l16] = sum[t][0];
+  }
+  __syncthreads();
+  #pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const int row = t * 16 + l16;
+    float mx = NEG_INF;
+    for (int k = 0; k < KG; k++) mx = __builtin_fmaxf(mx, stat[k * 32 + row]);
+    const float f = mx == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m[t] - mx);
+    #pragma unroll
+    for (int d = 0; d < DTH; d++)
+      if (dt0 + d < DT) *(f32x4*)&acc[(kg * 16 * RT + row) * HD + (dt0 + d) * 16 + lq * 4] = o[t][d] * f;
+  }
+  __syncthreads();
+  for (int u = tid; u < it.rows * (HD / 4); u += 256) {
+    const int row = u / (HD / 4), d = u % (HD / 4) * 4;
+    float mx = NEG_INF, l = 0.0f;
+    for (int k = 0; k < KG; k++) mx = __builtin_fmaxf(mx, stat[k * 32 + row]);
+    for (int k = 0; k < KG; k++) l += mx == NEG_INF ? 0.0f : stat[128 + k * 32 + row] * __builtin_amdgcn_exp2f(stat[k * 32 + row] - mx);
+    f32x4 v = *(const f32x4*)&acc[row * HD + d];
+    for (int k = 1; k < KG; k++) v += *(const f32x4*)&acc[(k * 16 * RT + row) * HD + d];
+    if (it.splits == 1) {
+      put4(a.o + out_at(it, g, row) + d, l == 0.0f ? (f32x4){0, 0, 0, 0} : v / l);
+    } else {
+      *(f32x4*)(part_sums(a, g, it.slot + it.split * it.rows + row) + d) = v;
+      if (d == 0) {
+        float* p = part_stats(a, g, it.slot + it.split * it.rows + row);
+        p[0] = mx, p[1] = l;
+      }
+    }
+  }
+  if (it.splits > 1) meet(a, it, g, 0, it.rows, it.rows);
+}
+
+// ── many rows: 32 a wave ──────────────────────────────────────────────────────────────────────────
+__device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, Stream& st, int t_first, int t_last, int lo_all, int hi_all, int full_lo, int full_hi) {
+  constexpr int NK = TK / 16;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
+  const int row0 = it.tile * (int)PR + wave * 32;
+  s16x8 qf[2][DSTEP];
+  int lo[2], hi[2];
+  #pragma unroll
+  for (int t = 0; t < 2; t++) {
+    int row = row0 + t * 16 + l16;
+    if (row >= it.rows) row = it.rows - 1;
+    const unsigned short* q = a.q + (QB + (it.start + row / REP) * Q0 + (g * REP + row % REP) * Q1);
+    read_row(q, lq, qf[t]);
+    hi[t] = clamp_pos(it.past + row / REP + 1);
+    lo[t] = W ? clamp_pos(it.past + row / REP + 1 - W) : 0;
+  }
+  // this wave's rows: what any and what all of them see
+  const int first = row0 < it.rows ? row0 : it.rows - 1, last = row0 + 31 < it.rows ? row0 + 31 : it.rows - 1;
+  const int wave_hi = clamp_pos(it.past + last / REP + 1), all_hi = clamp_pos(it.past + first / REP + 1);
+  const int wave_lo = W ? clamp_pos(it.past + first / REP + 1 - W) : 0, all_lo = W ? clamp_pos(it.past + last / REP + 1 - W) : 0;
+  const bool idle = row0 >= it.rows;
+  f32x4 o[2][DT], sum[2];
+  float m[2];
+  #pragma unroll
+  for (int t = 0; t < 2; t++) {
+    m[t] = NEG_INF, sum[t] = (f32x4){0, 0, 0, 0};
+    #pragma unroll
+    for (int d = 0; d < DT; d++) o[t][d] = (f32x4){0, 0, 0, 0};
+  }
+  begin(st, t_first, t_last, qf);
+  const short one = HALF ? (short)0x3C00 : (short)0x3F80;
+  const s16x8 ones = {one, one, one, one, one, one, one, one};
+  int buf = 0;
+  for (int i = t_first; i < t_last; i++) {
+    const int t0 = i * TK;
+    arrived(t_last - 1 - i);
+    if (i + STAGES - 1 < t_last) {
+      const int ahead = t0 + (STAGES - 1) * TK;
+      if (!st.covers(ahead)) {
+        __syncthreads();
+        st.pages_from(ahead / BS);
+        __syncthreads();
+      }
+      st.fetch(ahead, buf == 0 ? STAGES - 1 : buf - 1);
+    }
+    const bool any_hole = lds.holes;
+    unsigned long long odd = 0;
+    if (!(t0 >= full_lo && t0 + TK <= full_hi) || any_hole) {
+      // the tile is every wave's: cleaned by all, then used
+      if (tid == 0) lds.odd_keys = 0;
+      __syncthreads();
+      const unsigned long long mine = clean(st, buf, t0, 0, TK, 0, CH, lo_all, hi_all, tid, 256);
+      if (mine) atomicOr(&lds.odd_keys, mine);
+      __syncthreads();
+      odd = lds.odd_keys;
+    }
+    if (!idle && t0 < wave_hi && t0 + TK > wave_lo) {
+      const bool full = t0 >= all_lo && t0 + TK <= all_hi && !any_hole;
+      f32x4 s[2][NK];
+      #pragma unroll
+      for (int kt = 0; kt < NK; kt++) {
+        s[0][kt] = (f32x4){0, 0, 0, 0}, s[1][kt] = (f32x4){0, 0, 0, 0};
+        const int row = kt * 16 + l16;
+        #pragma unroll
+        for (int d = 0; d < DSTEP; d++) {
+          const s16x8 k = key_run(buf, row, d, lq);
+          s[0][kt] = mma32(k, qf[0][d], s[0][kt]);
+          s[1][kt] = mma32(k, qf[1][d], s[1][kt]);
+        }
+      }
+      s16x8 p[2][NK / 2][MANY_TERMS];
+      #pragma unroll
+      for (int t = 0; t < 2; t++) {
+        float factor;
+        weigh<NK>(st, s[t], full, any_hole, t0 + lq * 4, lo[t], hi[t], m[t], factor);
+        if (!__all(factor == 1.0f)) {
+          sum[t] *= factor;
+          #pragma unroll
+          for (int d = 0; d < DT; d++) o[t][d] *= factor;
+        }
+        if (odd) add_odd<NK, DT>(st, odd, t0, 0, s[t], o[t], 0, lq);
+        #pragma unroll
+        for (int ks = 0; ks < NK / 2; ks++)
+          #pragma unroll
+          for (int k = 0; k < MANY_TERMS; k++) {
+            const u32x2 x = pack(s[t][2 * ks]), y = pack(s[t][2 * ks + 1]);
+            p[t][ks][k] = __builtin_bit_cast(s16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3));
+            sum[t] = mma32(ones, p[t][ks][k], sum[t]);
+          }
+      }
+      #pragma unroll
+      for (int d = 0; d < DT; d++)
+        #pragma unroll
+        for (int ks = 0; ks < NK / 2; ks += 2) {
+          s16x4 x[4];
+          if (ks + 1 < NK / 2)
+            tr_read4(value_at(buf, ks * 32, d, l16, lq), value_at(buf, ks * 32 + 16, d, l16, lq), value_at(buf, ks * 32 + 32, d, l16, lq),
+                     value_at(buf, ks * 32 + 48, d, l16, lq), x[0], x[1], x[2], x[3]);
+          else {
+            tr_read1(value_at(buf, ks * 32, d, l16, lq), x[0]);
+            tr_read1(value_at(buf, ks * 32 + 16, d, l16, lq), x[1]);
+          }
+          #pragma unroll
+          for (int e = 0; e < 2; e++)
+            if (ks + e < NK / 2) {
+              const s16x8 v = __builtin_shufflevector(x[2 * e], x[2 * e + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+              #pragma unroll
+              for (int k = 0; k < MANY_TERMS; k++) {
+                o[0][d] = mma32(v, p[0][ks + e][k], o[0][d]);
+                o[1][d] = mma32(v, p[1][ks + e][k], o[1][d]);
+              }
+            }
+        }
+    }
+    buf = buf == STAGES - 1 ? 0 : buf + 1;
+  }
+  const int tile_rows = it.rows - it.tile * (int)PR < PR ? it.rows - it.tile * (int)PR : (int)PR;
+  #pragma unroll
+  for (int t = 0; t < 2; t++) {
+    const int r = wave * 32 + t * 16 + l16;
+    if (r >= tile_rows) continue;
+    const float l = sum[t][0];
+    if (it.splits == 1) {
+      const float f = l == 0.0f ? 0.0f : 1.0f / l;
+      #pragma unroll
+      for (int d = 0; d < DT; d++) put4(a.o + out_at(it, g, it.tile * (int)PR + r) + d * 16 + lq * 4, o[t][d] * f);
+    } else {
+      float* p = part_sums(a, g, it.slot + it.split * (int)PR + r);
+      #pragma unroll
+      for (int d = 0; d < DT; d++) *(f32x4*)(p + d * 16 + lq * 4) = o[t][d];
+      if (lq == 0) {
+        float* x = part_stats(a, g, it.slot + it.split * (int)PR + r);
+        x[0] = m[t], x[1] = l;
+      }
+    }
+  }
+  if (it.splits > 1) meet(a, it, g, it.tile * (int)PR, tile_rows, (int)PR);
+}
+
+extern "C" __global__ void __launch_bounds__(256, OCC) sanic_paged_attn(Args a) {
+  const int g = (int)(blockIdx.x % NKV);
+  Item it;
+  if (!find_item(a, (int)(blockIdx.x / NKV), it)) return;
+  // the rows of this workgroup, and the keys that any and that all of them see
+  const int r0 = it.tile < 0 ? 0 : it.tile * (int)PR, r1 = it.tile < 0 || r0 + PR > it.rows ? it.rows : r0 + (int)PR;
+  const long long p0 = it.past + r0 / REP, p1 = it.past + (r1 - 1) / REP;
+  const int hi_all = clamp_pos(p1 + 1), full_hi = clamp_pos(p0 + 1);
+  const int lo_all = W ? clamp_pos(p0 + 1 - W) : 0, full_lo = W ? clamp_pos(p1 + 1 - W) : 0;
+  const int k0 = lo_all / TK, k1 = lo_all < hi_all ? (hi_all + TK - 1) / TK : k0;
+  const int t_first = k0 + (int)((long long)(k1 - k0) * it.split / it.splits), t_last = k0 + (int)((long long)(k1 - k0) * (it.split + 1) / it.splits);
+  Stream st{a, a.tables + (long long)it.b * M, g, lo_all / (int)BS, (hi_all - 1) / (int)BS, 0, a.k + (KB + g * K1), a.v + (VB + g * V1)};
+  if (it.tile >= 0) {
+    if (PITEMS) many_rows(a, it, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
+  } else if (it.rows <= 16) {
+    few_rows<1>(a, it, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
+  } else {
+    few_rows<2>(a, it, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
+  }
+}
+)SRC";
+
+// The matrix-core kernel takes queries and caches of one 16-bit type whose rows are runs of a multiple
+// of 16 elements, in units of 16 bytes.
+static bool mfma_takes(const OperandView& q, const OperandView& k, const OperandView& v) {
+    const int64_t HD = q.extent[2];
+    if (q.dtype != k.dtype || (q.dtype != SANIC_BF16 && q.dtype != SANIC_F16) || HD % 16 || HD > 256) return false;
+    for (const OperandView* o : {&q, &k, &v}) {
+        if (o->stride.back() != 1 || o->base % 8) return false;
+        for (size_t j = 0; j + 1 < o->stride.size(); j++)
+            if (o->stride[j] % 8) return false;
+    }
+    return true;
+}
+
 LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st, int64_t& scratch) {
-    (void)scratch;
     OperandView q, k, v;
     operand_view(d, st.leaf[0], q), operand_view(d, st.leaf[1], k), operand_view(d, st.leaf[2], v);
     const int64_t T = q.extent[0], NH = q.extent[1], HD = q.extent[2], NB = k.extent[0], NKV = k.extent[1], BS = k.extent[2];
     const sanic_node& tables = d->nodes[st.leaf[3]];
+    const int64_t B = tables.shape[0], M = tables.shape[1], REP = NH / NKV;
+    const double scale = d->nodes[st.leaf[6]].value;
     std::string c;
-    c += constant("T", T) + constant("NH", NH) + constant("HD", HD) + constant("NB", NB) + constant("BS", BS) + constant("REP", NH / NKV);
-    c += constant("B", tables.shape[0]) + constant("M", tables.shape[1]) + constant("W", st.stream);
-    c += constant("DQ", q.dtype) + constant("DC", k.dtype) + constant("DO", st.out_dtype) + "constexpr float SCALE = " + flit(d->nodes[st.leaf[6]].value) + ";\n";
+    c += constant("T", T) + constant("NH", NH) + constant("HD", HD) + constant("NB", NB) + constant("BS", BS) + constant("REP", REP);
+    c += constant("B", B) + constant("M", M) + constant("W", st.stream) + constant("NKV", NKV);
+    c += constant("DQ", q.dtype) + constant("DC", k.dtype) + constant("DO", st.out_dtype) + "constexpr float SCALE = " + flit(scale) + ";\n";
     auto strides = [&](const char* n, const OperandView& o) {
         for (size_t j = 0; j < o.stride.size(); j++) c += constant((std::string(n) + std::to_string(j)).c_str(), o.stride[j]);
         c += constant((std::string(n) + "B").c_str(), o.base);
     };
     strides("Q", q), strides("K", k), strides("V", v);
     LoweredStage L;
-    L.kernel_kind = "operator:paged_attn[plain]";
-    L.source = std::string(kPrelude) + kElement + c + kPlain;
     Launch ln{"sanic_paged_attn", "", dim3((unsigned)((T * NH + 3) / 4)), dim3(256), 0, {}};
     for (int b : {q.buffer, k.buffer, v.buffer, tables.buffer, d->nodes[st.leaf[4]].buffer, d->nodes[st.leaf[5]].buffer, st.out_buffer})
         ln.args.push_back({Arg::BUF, b});
+    if (!mfma_takes(q, k, v) || !std::isfinite(scale)) {
+        L.kernel_kind = "operator:paged_attn[plain]";
+        L.source = std::string(kPrelude) + kElement + c + kPlain;
+        L.launches.push_back(ln);
+        return L;
+    }
+    // tiles: three of up to 8 KB for the keys and as much for the values leave three workgroups a CU
+    const int64_t TK = HD <= 64 ? 64 : 32, STAGES = HD <= 128 ? 3 : 2, OCC = HD <= 128 ? 3 : HD <= 192 ? 2 : 1;
+    const int64_t PR = 128, DR = 32, MEET = 4096;
+    const int64_t slots = 256 * OCC;
+    // items a key head: twice the workgroups that run at once
+    const int64_t live = std::min(B, T), few = std::max<int64_t>(1, 2 * slots / NKV);
+    const int64_t budget = (lean_scratch() ? int64_t(1) << 20 : int64_t(10) << 20) / (NKV * (HD + 2) * 4);
+    const int64_t DROWS = std::min((few + live) * std::min(DR, T * REP), budget);
+    const int64_t tiles = T * REP > DR ? T * REP / PR + std::min(live, T * REP / (DR + 1)) : 0;
+    const int64_t PSPLIT = tiles ? std::min(2 * slots / NKV, budget / PR) : 0;
+    const int64_t SLOTS = DROWS + PSPLIT * PR;
+    c += constant("TK", TK) + constant("STAGES", STAGES) + constant("OCC", OCC) + constant("PR", PR) + constant("DR", DR) + constant("MEET", MEET);
+    c += constant("DTARGET", few) + constant("DROWS", DROWS) + constant("PITEMS", tiles > 0) + constant("PSPLIT", PSPLIT) + constant("SLOTS", SLOTS);
+    c += constant("PAGES", 512) + constant("FLIP", scale < 0) + "constexpr float C2 = " + flit(std::fabs(scale) * 1.4426950408889634) + ";\n";
+    // Weights take the 16 bits of the matrix cores' operands. Few rows are bound by the cache's bytes: a
+    // second term (what the rounding left) costs nothing there. Many rows are bound by the products and
+    // keep one term: half a step of relative error a weight, of both signs, in sums divided by the same
+    // rounded weights' sum. An f32 output gets 24 bits from three terms (f16: 22 from two, and the rest).
+    c += constant("FEW_TERMS", st.out_dtype == SANIC_F32 ? 3 : 2) + constant("MANY_TERMS", st.out_dtype == SANIC_F32 ? 3 : 1);
+    L.kernel_kind = "operator:paged_attn[mfma]";
+    L.source = std::string(kPrelude) + kElement + c + kMfma;
+    ln.grid = dim3((unsigned)(NKV * (few + live + std::max(tiles, PSPLIT))));
+    ln.args.push_back({Arg::SCRATCH, shared_scratch(scratch, NKV * SLOTS * (HD + 2) * 4)});
+    ln.args.push_back({Arg::COUNTERS, shared_counters((B + PSPLIT / 2 + 1) * NKV)});
     L.launches.push_back(ln);
     return L;
 }

@@ -421,6 +421,33 @@ def test_paged_attention_nan_in_sight(dev, new):
     assert np.isnan(got[:new]).all() and np.isfinite(got[new:]).all()
 
 
+@pytest.mark.parametrize("dtype", [ir.BF16, ir.F16])
+@pytest.mark.parametrize("HD", [64, 128, 80])
+@pytest.mark.parametrize("new,at", [(6, 4), (6, 0), (90, 61), (200, 130)])
+def test_paged_attention_not_finite_behind_some_rows(dev, dtype, HD, new, at):
+    """What is not finite at one of the step's own tokens reaches the rows from there on, and no
+    element of the rows before it (0 · NaN would, were the masked keys multiplied)."""
+    for value in (np.nan, np.inf, -np.inf):
+        t = Batch(past=[70], new=[new], NKV=2, rep=3, HD=HD, BS=16, dq=dtype)
+        where = (int(t.tables[0, (70 + at) // 16]), slice(None), (70 + at) % 16)
+        t.vc[where + (5,)] = value
+        t.kc[where + (3,)] = np.nan if at % 2 else 1.0     # a key too: its score is NaN where it is seen
+        p = t.program()
+        bufs = bind(dev, p, t.values())
+        exe = dev.prepare(p)
+        exe.execute_static(bufs)
+        got = read(p, bufs, "o")
+        clean = Batch(past=[70], new=[new], NKV=2, rep=3, HD=HD, BS=16, dq=dtype)
+        clean.starts = np.array([0, at])
+        clean.check(got, exe.stage_kernel(0))
+        late = got[at:]
+        if at % 2:
+            assert np.isnan(late).all()
+        else:
+            assert np.isfinite(np.delete(late, 5, axis=2)).all()
+            assert np.isnan(late[..., 5]).all() if np.isnan(value) else (late[..., 5] == value).all()
+
+
 # ── verification of drafts ───────────────────────────────────────────────────
 
 def verify_program(T, B, V, dp, dq):

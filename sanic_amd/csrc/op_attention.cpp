@@ -36,7 +36,7 @@ extern "C" __global__ void __launch_bounds__(256) sanic_paged_attn(Args a) {
   }
   if (r < a.starts[b] || r >= a.starts[b + 1]) return;
   const long long p = (long long)a.past[b] + (r - a.starts[b]);
-  const long long end = p + 1 < M * BS ? p + 1 : M * BS;
+  const long long most = (long long)M * BS, end = p + 1 < most ? p + 1 : most;
   const long long lo = W && p + 1 > W ? p + 1 - W : 0;
   for (int e = lane; e < HD; e += 64) q_of[wave][e] = sanic_get<DQ>(a.q[QB + r * Q0 + h * Q1 + e * Q2]) * SCALE;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -114,12 +114,11 @@ typedef sanic_elem<DO>::T o_t;
 struct Args { const unsigned short *q, *k, *v; const unsigned *tables, *starts, *past; o_t* o; float* part; unsigned* counts; };
 
 constexpr bool HALF = DQ == 2;
-constexpr int CH = HD / 8;                       // 16-byte chunks of a key's row
-constexpr int DSTEP = (HD + 31) / 32;            // products over 32 head dims, the last one's upper half 0 if HD is odd times 16
-constexpr int DT = HD / 16;
-constexpr int LOADS = (TK * CH + 255) / 256;     // 16-byte loads a lane for a tile's keys, and its values
-constexpr int TILE = LOADS * 256 * 8;            // elements of a staged tile, the last lanes' surplus included
-constexpr int KG = TK / 16, DH = 4 / KG, DTH = (DT + DH - 1) / DH;
+constexpr int CH = HD / 8, CG = (CH + 3) / 4;    // 16-byte chunks of a key's row, and 64-byte groups of them
+constexpr int DSTEP = CG, DT = HD / 16;          // products over 32 head dims; value tiles of 16 dims
+constexpr int LOADS = (TK / 16 * CG + 3) / 4;    // 16-byte loads a lane for a tile's keys, and its values
+constexpr int TILE = LOADS * 4 * 512;            // elements of a staged tile, surplus loads included
+constexpr int KG = TK / 16, DH = 4 / KG, DTH = DH == 1 ? DT : (DT + 3) / 4 * 2;
 constexpr int MBS = M * BS;                      // positions a block table can hold
 constexpr float NEG_INF = -__builtin_huge_valf();
 
@@ -151,21 +150,17 @@ __device__ __forceinline__ u32x2 pack(f32x4& x) {
 __device__ __forceinline__ float quad_max(float v) {  // over the 4 lanes of a row's column
   return sanic_rows_max(v);
 }
-// a chunk's place in its row of the staged tile: rotated by the row, so that the 16 rows a wave reads
-// at one dim lie in different banks
-__device__ __forceinline__ int spot(int row, int c) {
-  if constexpr ((CH & (CH - 1)) == 0 && CH >= 4) return c ^ (row & (CH < 16 ? CH - 1 : 15));
-  else return (c + row) % CH;
-}
-__device__ __forceinline__ int chunk_at(int row, int at) {  // its inverse
-  if constexpr ((CH & (CH - 1)) == 0 && CH >= 4) return at ^ (row & (CH < 16 ? CH - 1 : 15));
-  else return (at + CH - row % CH) % CH;
-}
+// A staged tile is made of blocks of 16 rows × 4 chunks (1 KB, one load a lane: 64 contiguous bytes of
+// each row), [row group][chunk group]; inside a block the chunks of a row are swapped by the row, so
+// that rows a wave reads at one dim lie in different banks, and a lane's place in a block is the same
+// in all of them: reads differ by constant offsets.
+__device__ __forceinline__ int in_block(int row, int c) { return ((row & 15) * 4 + ((c & 3) ^ (row >> 1 & 3))) * 8; }
+__device__ __forceinline__ int spot(int row, int c) { return ((row >> 4) * CG + (c >> 2)) * 512 + in_block(row, c); }
 __device__ __forceinline__ int clamp_pos(long long p) { return p < 0 ? 0 : p > MBS ? MBS : (int)p; }
 
 // (one object: with several, the compiler waits for every load into LDS before any read of it)
 __shared__ struct {
-  __attribute__((aligned(16))) unsigned short ring[STAGES][2][TILE];
+  __attribute__((aligned(1024))) unsigned short ring[STAGES][2][TILE];
   unsigned pages[PAGES];
   unsigned long long odd_keys;
   int holes, last_arrival;
@@ -295,25 +290,31 @@ struct Stream {
   __device__ __forceinline__ bool covers(int t0) const { return t0 / BS >= base && (t0 + TK - 1) / BS < base + PAGES; }
   __device__ __forceinline__ void fetch(int t0, int buf) const {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = lane >> 2, c = (lane & 3) ^ (row >> 1 & 3);
     #pragma unroll
     for (int u = 0; u < LOADS; u++) {
-      const int i = (u * 4 + wave) * 64 + lane;
-      int row = i / CH;
-      const int c = chunk_at(row, i % CH) * 8;
-      if (TK * CH % 256 && row >= TK) row = TK - 1;
-      const int key = t0 + row;
+      const int n = u * 4 + wave;
+      int group = n / CG, chunk = n % CG * 4 + c;
+      if (TK / 16 * CG % 4 && group >= TK / 16) group = TK / 16 - 1;
+      if (CH % 4 && chunk >= CH) chunk = CH - 1;    // (the query is 0 there)
+      const int key = t0 + group * 16 + row;
       const unsigned page = lds.pages[key / BS - base];
       const long long pg = page < NB ? page : 0, in = key % BS;    // a page that is none is read as block 0 and masked
-      const unsigned short* kp = k + (pg * K0 + in * K2 + c);
-      const unsigned short* vp = v + (pg * V0 + in * V2 + c);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)kp, (__attribute__((address_space(3))) void*)&lds.ring[buf][0][(u * 4 + wave) * 512], 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vp, (__attribute__((address_space(3))) void*)&lds.ring[buf][1][(u * 4 + wave) * 512], 16, 0, 0);
+      const unsigned short* kp = k + (pg * K0 + in * K2 + chunk * 8);
+      const unsigned short* vp = v + (pg * V0 + in * V2 + chunk * 8);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)kp, (__attribute__((address_space(3))) void*)&lds.ring[buf][0][n * 512], 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vp, (__attribute__((address_space(3))) void*)&lds.ring[buf][1][n * 512], 16, 0, 0);
     }
   }
-  // the key is in the pool (asked where a tile has keys that are not)
-  __device__ __forceinline__ bool there(int key) const {
-    const int p = key / BS;
-    return p >= first_page && p <= last_page && table[p] < NB;
+  // the keys of a tile that are in no block of the pool, a bit each
+  __device__ __forceinline__ unsigned long long missing(int t0) const {
+    unsigned long long out = 0;
+    for (int p = t0 / BS; p <= (t0 + TK - 1) / BS; p++) {
+      if (p < first_page || p > last_page || table[p] < NB) continue;
+      const int from = p * BS - t0, to = from + BS;
+      for (int r = from > 0 ? from : 0; r < (to < TK ? to : TK); r++) out |= 1ull << r;
+    }
+    return out;
   }
 };
 
@@ -346,31 +347,36 @@ __device__ __forceinline__ void arrived(int left) {
   else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-__device__ __forceinline__ s16x8 key_run(int buf, int row, int step, int lq) {
-  const int c = step * 4 + lq;
-  if (HD % 32 == 0 || c < CH) return *(const s16x8*)&lds.ring[buf][0][row * HD + spot(row, c) * 8];
-  return (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
+__device__ __forceinline__ s16x8 key_run(int buf, int group, int step, int l16, int lq) {
+  return *(const s16x8*)&lds.ring[buf][0][(group * CG + step) * 512 + in_block(l16, lq)];
 }
-// LDS address of a lane's part of a transposed read of 16 keys (from row `row0`) × 16 value dims
-__device__ __forceinline__ unsigned value_at(int buf, int row0, int dt, int l16, int lq) {
-  const int row = row0 + lq * 4 + (l16 >> 2), col = dt * 16 + (l16 & 3) * 4;
-  return (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned short*)&lds.ring[buf][1][row * HD + spot(row, col >> 3) * 8 + (col & 7)];
+// Transposed reads of 16 keys × 16 value dims: a lane gets 4 keys of one dim. A lane's place in a block
+// for an even tile of dims; for an odd one it is 32 bytes further or back (two chunks, swapped alike).
+__device__ __forceinline__ unsigned value_at(int buf, int l16, int lq) {
+  return (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned short*)&lds.ring[buf][1][in_block(lq * 4 + (l16 >> 2), l16 >> 1 & 1) + (l16 & 1) * 4];
 }
-// Transposed reads (a lane gets 4 keys of one value dim), waited for in the same statement: the
-// compiler takes an asm output as written at once.
-__device__ __forceinline__ void tr_read4(unsigned a0, unsigned a1, unsigned a2, unsigned a3, s16x4& r0, s16x4& r1, s16x4& r2, s16x4& r3) {
-  asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %2, %6\n\tds_read_b64_tr_b16 %3, %7\n\ts_waitcnt lgkmcnt(0)"
-               : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3) : "v"(a0), "v"(a1), "v"(a2), "v"(a3) : "memory");
+// (waited for in the same statement: the compiler takes an asm output as written at once)
+template <int I0, int I1>
+__device__ __forceinline__ void tr_read4(unsigned even, s16x4& r0, s16x4& r1, s16x4& r2, s16x4& r3) {
+  asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %5 offset:%6\n\t"
+               "ds_read_b64_tr_b16 %2, %4 offset:%7\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3) : "v"(even), "v"(even ^ 32u), "n"(I0), "n"(I1) : "memory");
 }
-__device__ __forceinline__ void tr_read1(unsigned a0, s16x4& r0) {
-  asm volatile("ds_read_b64_tr_b16 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(r0) : "v"(a0) : "memory");
+template <int I0, int I1, int I2, int I3>
+__device__ __forceinline__ void tr_read8(unsigned even, s16x4 (&r)[8]) {
+  asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%10\n\tds_read_b64_tr_b16 %1, %9 offset:%10\n\t"
+               "ds_read_b64_tr_b16 %2, %8 offset:%11\n\tds_read_b64_tr_b16 %3, %9 offset:%11\n\t"
+               "ds_read_b64_tr_b16 %4, %8 offset:%12\n\tds_read_b64_tr_b16 %5, %9 offset:%12\n\t"
+               "ds_read_b64_tr_b16 %6, %8 offset:%13\n\tds_read_b64_tr_b16 %7, %9 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+               : "v"(even), "v"(even ^ 32u), "n"(I0), "n"(I1), "n"(I2), "n"(I3) : "memory");
 }
 __device__ __forceinline__ bool odd_value(unsigned short x) { return HALF ? (x & 0x7C00) == 0x7C00 : (x & 0x7F80) == 0x7F80; }
 
-// One column of scores into weights: s holds the products of keys key0 + 16·kt + r of row [lo, hi) and
-// leaves as 2^(t − m). `factor` is what the row's earlier sums are scaled by.
+// One column of scores into weights: s holds the products of the tile's keys row0 + 16·kt + r, of which
+// the row sees those in [lo, hi) that are no holes, and leaves as 2^(t − m). `factor` is what the row's earlier sums are scaled by.
 template <int N>
-__device__ __forceinline__ void weigh(const Stream& st, f32x4 (&s)[N], bool full, bool any_hole, int key0, int lo, int hi, float& m, float& factor) {
+__device__ __forceinline__ void weigh(f32x4 (&s)[N], bool full, unsigned long long holes, int row0, int lo, int hi, float& m, float& factor) {
   float top = NEG_INF;
   if (full) {
     #pragma unroll
@@ -381,9 +387,8 @@ __device__ __forceinline__ void weigh(const Stream& st, f32x4 (&s)[N], bool full
     for (int kt = 0; kt < N; kt++)
       #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int key = key0 + kt * 16 + r;
-        bool seen = key >= lo && key < hi;
-        if (any_hole && seen) seen = st.there(key);
+        const int key = row0 + kt * 16 + r;
+        const bool seen = key >= lo && key < hi && !(holes >> key & 1);
         s[kt][r] = seen ? s[kt][r] * C2 : NEG_INF;
         top = __builtin_fmaxf(top, s[kt][r]);
       }
@@ -405,20 +410,22 @@ __device__ __forceinline__ void weigh(const Stream& st, f32x4 (&s)[N], bool full
 
 // Values that nobody in the workgroup sees become 0 (0·NaN would reach every row of the product);
 // where one that is seen is not finite, its key's bit is returned, and it is 0 in the tile: add_odd
-// adds it to the rows that see it. Rows [row0, row0 + rows) × chunks [c0, c0 + chunks), 64 lanes.
-__device__ __forceinline__ unsigned long long clean(const Stream& st, int buf, int t0, int row0, int rows, int c0, int chunks, int lo, int hi, int part, int parts) {
+// adds it to the rows that see it. Rows [row0, row0 + rows) × chunks [c0, c0 + chunks), of which any row
+// sees [lo, hi) (rows counted from the tile's first key).
+__device__ __forceinline__ unsigned long long clean(int buf, unsigned long long holes, int row0, int rows, int c0, int chunks, int lo, int hi, int part, int parts) {
   unsigned long long odd = 0;
   for (int i = part; i < rows * chunks; i += parts) {
-    const int row = row0 + i / chunks, c = c0 + i % chunks, key = t0 + row;
-    s16x8* p = (s16x8*)&lds.ring[buf][1][row * HD + spot(row, c) * 8];
+    const int row = row0 + i / chunks;
+    s16x8* p = (s16x8*)&lds.ring[buf][1][spot(row, c0 + i % chunks)];
     s16x8 x = *p;
-    bool dead = key < lo || key >= hi, change = false;
-    if (!dead && lds.holes) dead = !st.there(key);
+    const bool dead = row < lo || row >= hi || (holes >> row & 1);
+    bool change = dead;
     #pragma unroll
     for (int e = 0; e < 8; e++) {
       const bool o = odd_value((unsigned short)x[e]);
+      change |= o;
       if (o && !dead) odd |= 1ull << row;
-      if (o || dead) x[e] = 0, change = true;
+      if (o || dead) x[e] = 0;
     }
     if (change) *p = x;
   }
@@ -437,15 +444,19 @@ __device__ __forceinline__ void add_odd(const Stream& st, unsigned long long odd
         if (rel + kt * 16 + lq * 4 + r == row) x = w[kt][r];
     x = sanic_rows_sum(x);
     const unsigned page = st.table[key / BS];
-    if (page >= NB) continue;
     const unsigned short* v = st.v + ((long long)page * V0 + key % BS * V2);
     #pragma unroll
-    for (int d = 0; d < D; d++)
+    for (int d = 0; d < D; d++) {
+      const int col = (dt0 + d) * 16 + lq * 4;
+      if (col >= HD) continue;
+      struct __attribute__((packed, aligned(4))) run { unsigned short e[4]; };
+      const run y = *(const run*)(v + col);
       #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int col = (dt0 + d) * 16 + lq * 4 + r;
-        if (col < HD && odd_value(v[col]) && x != 0.0f) o[d][r] += x * sanic_get<DQ>(__builtin_bit_cast(sanic_elem<DQ>::T, v[col]));
+        const float z = x * sanic_get<DQ>(__builtin_bit_cast(sanic_elem<DQ>::T, y.e[r]));
+        o[d][r] += odd_value(y.e[r]) && x != 0.0f ? z : 0.0f;
       }
+    }
   }
 }
 
@@ -540,6 +551,13 @@ __device__ __forceinline__ void read_row(const unsigned short* q, int lq, s16x8 
   }
 }
 
+// the values of 16 keys, four tiles of dims at a time (a last tile's read may be of the tile before it)
+template <int D>
+__device__ __forceinline__ void few_values(unsigned at, s16x4 (&vt)[(DTH + 3) / 4 * 4]) {
+  tr_read4<D / 2 * 1024, (D / 2 + 1 < CG ? D / 2 + 1 : D / 2) * 1024>(at, vt[D], vt[D + 1], vt[D + 2], vt[D + 3]);
+  if constexpr (D + 4 < DTH) few_values<D + 4>(at, vt);
+}
+
 // ── few rows: the waves split the tile's keys ─────────────────────────────────────────────────────
 template <int RT>
 __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int g, Stream& st, int t_first, int t_last, int lo_all, int hi_all, int full_lo, int full_hi) {
@@ -580,42 +598,29 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int g, S
       }
       st.fetch(ahead, buf == 0 ? STAGES - 1 : buf - 1);
     }
-    const bool any_hole = lds.holes, full = t0 >= full_lo && t0 + TK <= full_hi && !any_hole;
+    const unsigned long long holes = lds.holes ? st.missing(t0) : 0;
+    const bool full = t0 >= full_lo && t0 + TK <= full_hi && !holes;
     unsigned long long odd = 0;
     if (!full) {
       const int c0 = dt0 * 2, c1 = (dt0 + DTH) * 2 < CH ? (dt0 + DTH) * 2 : CH;
-      odd = clean(st, buf, t0, kg * 16, 16, c0, c1 - c0, lo_all, hi_all, lane, 64);
+      odd = clean(buf, holes, kg * 16, 16, c0, c1 - c0, lo_all - t0, hi_all - t0, lane, 64);
       for (int x = 1; x < 64; x <<= 1) odd |= __shfl_xor(odd, x);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    s16x4 vt[DTH];
+    s16x4 vt[(DTH + 3) / 4 * 4];
     #pragma unroll
     for (int t = 0; t < RT; t++) {
       f32x4 s[1] = {{0, 0, 0, 0}};
-      const int row = kg * 16 + l16;
       #pragma unroll
-      for (int d = 0; d < DSTEP; d++) s[0] = mma32(key_run(buf, row, d, lq), qf[t][d], s[0]);
+      for (int d = 0; d < DSTEP; d++) s[0] = mma32(key_run(buf, kg, d, l16, lq), qf[t][d], s[0]);
       float factor;
-      weigh<1>(st, s, full, any_hole, t0 + kg * 16 + lq * 4, lo[t], hi[t], m[t], factor);
+      weigh<1>(s, full, holes, kg * 16 + lq * 4, lo[t] - t0, hi[t] - t0, m[t], factor);
       if (!__all(factor == 1.0f)) {
         sum[t] *= factor;
         #pragma unroll
         for (int d = 0; d < DTH; d++) o[t][d] *= factor;
       }
-      if (t == 0) {
-        #pragma unroll
-        for (int d = 0; d < DTH; d += 4) {
-          unsigned at[4];
-          #pragma unroll
-          for (int e = 0; e < 4; e++) at[e] = value_at(buf, kg * 16, dt0 + (d + e < DTH ? d + e : d) < DT ? dt0 + (d + e < DTH ? d + e : d) : 0, l16, lq);
-          if (d + 3 < DTH) tr_read4(at[0], at[1], at[2], at[3], vt[d], vt[d + 1], vt[d + 2], vt[d + 3]);
-          else {
-            #pragma unroll
-            for (int e = 0; e < 4; e++)
-              if (d + e < DTH) tr_read1(at[e], vt[d + e]);
-          }
-        }
-      }
+      if (t == 0) few_values<0>(value_at(buf, l16, lq) + (kg * CG + (dt0 >> 1)) * 1024, vt);
       if (odd) add_odd<1, DTH>(st, odd, t0, kg * 16, s, o[t], dt0, lq);
       #pragma unroll
       for (int k = 0; k < FEW_TERMS; k++) {
@@ -667,6 +672,31 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int g, S
   if (it.splits > 1) meet(a, it, g, 0, it.rows, it.rows);
 }
 
+// Oᵀ += Vᵀ·P over the tile, eight reads (all keys of two or four tiles of dims) at a time
+template <int D>
+__device__ __forceinline__ void many_values(unsigned at, const s16x8 (&p)[2][TK / 32][MANY_TERMS], f32x4 (&o)[2][DT]) {
+  constexpr int KS = TK / 32, G = 8 / (TK / 16);    // dim tiles a group
+  constexpr int B0 = D / 2, B1 = D / 2 + 1 < CG ? D / 2 + 1 : D / 2;
+  s16x4 r[8];
+  if constexpr (KS == 2) tr_read8<B0 * 1024, (CG + B0) * 1024, (2 * CG + B0) * 1024, (3 * CG + B0) * 1024>(at, r);
+  else tr_read8<B0 * 1024, (CG + B0) * 1024, B1 * 1024, (CG + B1) * 1024>(at, r);
+  #pragma unroll
+  for (int e = 0; e < G; e++) {
+    if (D + e >= DT) break;
+    #pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+      const int i = KS == 2 ? 4 * ks + e : 4 * (e / 2) + e % 2;
+      const s16x8 v = __builtin_shufflevector(r[i], r[i + 2], 0, 1, 2, 3, 4, 5, 6, 7);
+      #pragma unroll
+      for (int k = 0; k < MANY_TERMS; k++) {
+        o[0][D + e] = mma32(v, p[0][ks][k], o[0][D + e]);
+        o[1][D + e] = mma32(v, p[1][ks][k], o[1][D + e]);
+      }
+    }
+  }
+  if constexpr (D + G < DT) many_values<D + G>(at, p, o);
+}
+
 // ── many rows: 32 a wave ──────────────────────────────────────────────────────────────────────────
 __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, Stream& st, int t_first, int t_last, int lo_all, int hi_all, int full_lo, int full_hi) {
   constexpr int NK = TK / 16;
@@ -712,27 +742,26 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
       }
       st.fetch(ahead, buf == 0 ? STAGES - 1 : buf - 1);
     }
-    const bool any_hole = lds.holes;
+    const unsigned long long holes = lds.holes ? st.missing(t0) : 0;
     unsigned long long odd = 0;
-    if (!(t0 >= full_lo && t0 + TK <= full_hi) || any_hole) {
+    if (!(t0 >= full_lo && t0 + TK <= full_hi) || holes) {
       // the tile is every wave's: cleaned by all, then used
       if (tid == 0) lds.odd_keys = 0;
       __syncthreads();
-      const unsigned long long mine = clean(st, buf, t0, 0, TK, 0, CH, lo_all, hi_all, tid, 256);
+      const unsigned long long mine = clean(buf, holes, 0, TK, 0, CH, lo_all - t0, hi_all - t0, tid, 256);
       if (mine) atomicOr(&lds.odd_keys, mine);
       __syncthreads();
       odd = lds.odd_keys;
     }
     if (!idle && t0 < wave_hi && t0 + TK > wave_lo) {
-      const bool full = t0 >= all_lo && t0 + TK <= all_hi && !any_hole;
+      const bool full = t0 >= all_lo && t0 + TK <= all_hi && !holes;
       f32x4 s[2][NK];
       #pragma unroll
       for (int kt = 0; kt < NK; kt++) {
         s[0][kt] = (f32x4){0, 0, 0, 0}, s[1][kt] = (f32x4){0, 0, 0, 0};
-        const int row = kt * 16 + l16;
         #pragma unroll
         for (int d = 0; d < DSTEP; d++) {
-          const s16x8 k = key_run(buf, row, d, lq);
+          const s16x8 k = key_run(buf, kt, d, l16, lq);
           s[0][kt] = mma32(k, qf[0][d], s[0][kt]);
           s[1][kt] = mma32(k, qf[1][d], s[1][kt]);
         }
@@ -741,7 +770,7 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
       #pragma unroll
       for (int t = 0; t < 2; t++) {
         float factor;
-        weigh<NK>(st, s[t], full, any_hole, t0 + lq * 4, lo[t], hi[t], m[t], factor);
+        weigh<NK>(s[t], full, holes, lq * 4, lo[t] - t0, hi[t] - t0, m[t], factor);
         if (!__all(factor == 1.0f)) {
           sum[t] *= factor;
           #pragma unroll
@@ -757,29 +786,7 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
             sum[t] = mma32(ones, p[t][ks][k], sum[t]);
           }
       }
-      #pragma unroll
-      for (int d = 0; d < DT; d++)
-        #pragma unroll
-        for (int ks = 0; ks < NK / 2; ks += 2) {
-          s16x4 x[4];
-          if (ks + 1 < NK / 2)
-            tr_read4(value_at(buf, ks * 32, d, l16, lq), value_at(buf, ks * 32 + 16, d, l16, lq), value_at(buf, ks * 32 + 32, d, l16, lq),
-                     value_at(buf, ks * 32 + 48, d, l16, lq), x[0], x[1], x[2], x[3]);
-          else {
-            tr_read1(value_at(buf, ks * 32, d, l16, lq), x[0]);
-            tr_read1(value_at(buf, ks * 32 + 16, d, l16, lq), x[1]);
-          }
-          #pragma unroll
-          for (int e = 0; e < 2; e++)
-            if (ks + e < NK / 2) {
-              const s16x8 v = __builtin_shufflevector(x[2 * e], x[2 * e + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-              #pragma unroll
-              for (int k = 0; k < MANY_TERMS; k++) {
-                o[0][d] = mma32(v, p[0][ks + e][k], o[0][d]);
-                o[1][d] = mma32(v, p[1][ks + e][k], o[1][d]);
-              }
-            }
-        }
+      many_values<0>(value_at(buf, l16, lq), p, o);
     }
     buf = buf == STAGES - 1 ? 0 : buf + 1;
   }
@@ -849,8 +856,9 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     const int64_t B = tables.shape[0], M = tables.shape[1], REP = NH / NKV;
     const double scale = d->nodes[st.leaf[6]].value;
     std::string c;
-    c += constant("T", T) + constant("NH", NH) + constant("HD", HD) + constant("NB", NB) + constant("BS", BS) + constant("REP", REP);
-    c += constant("B", B) + constant("M", M) + constant("W", st.stream) + constant("NKV", NKV);
+    auto number = [](const char* n, int64_t v) { return std::string("constexpr int ") + n + " = " + std::to_string(v) + ";\n"; };
+    c += number("T", T) + number("NH", NH) + number("HD", HD) + constant("NB", NB) + number("BS", BS) + number("REP", REP);
+    c += number("B", B) + number("M", M) + constant("W", st.stream) + number("NKV", NKV);
     c += constant("DQ", q.dtype) + constant("DC", k.dtype) + constant("DO", st.out_dtype) + "constexpr float SCALE = " + flit(scale) + ";\n";
     auto strides = [&](const char* n, const OperandView& o) {
         for (size_t j = 0; j < o.stride.size(); j++) c += constant((std::string(n) + std::to_string(j)).c_str(), o.stride[j]);
@@ -868,7 +876,7 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
         return L;
     }
     // tiles: three of up to 8 KB for the keys and as much for the values leave three workgroups a CU
-    const int64_t TK = HD <= 64 ? 64 : 32, STAGES = HD <= 128 ? 3 : 2, OCC = HD <= 128 ? 3 : HD <= 192 ? 2 : 1;
+    const int64_t TK = HD <= 64 ? 64 : 32, STAGES = HD <= 128 ? 3 : 2, OCC = HD <= 64 ? 3 : HD <= 192 ? 2 : 1;
     const int64_t PR = 128, DR = 32, MEET = 4096;
     const int64_t slots = 256 * OCC;
     // items a key head: twice the workgroups that run at once
@@ -878,14 +886,14 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     const int64_t tiles = T * REP > DR ? T * REP / PR + std::min(live, T * REP / (DR + 1)) : 0;
     const int64_t PSPLIT = tiles ? std::min(2 * slots / NKV, budget / PR) : 0;
     const int64_t SLOTS = DROWS + PSPLIT * PR;
-    c += constant("TK", TK) + constant("STAGES", STAGES) + constant("OCC", OCC) + constant("PR", PR) + constant("DR", DR) + constant("MEET", MEET);
-    c += constant("DTARGET", few) + constant("DROWS", DROWS) + constant("PITEMS", tiles > 0) + constant("PSPLIT", PSPLIT) + constant("SLOTS", SLOTS);
-    c += constant("PAGES", 512) + constant("FLIP", scale < 0) + "constexpr float C2 = " + flit(std::fabs(scale) * 1.4426950408889634) + ";\n";
+    c += number("TK", TK) + number("STAGES", STAGES) + number("OCC", OCC) + number("PR", PR) + number("DR", DR) + number("MEET", MEET);
+    c += number("DTARGET", few) + number("DROWS", DROWS) + number("PITEMS", tiles > 0) + number("PSPLIT", PSPLIT) + number("SLOTS", SLOTS);
+    c += number("PAGES", 512) + number("FLIP", scale < 0) + "constexpr float C2 = " + flit(std::fabs(scale) * 1.4426950408889634) + ";\n";
     // Weights take the 16 bits of the matrix cores' operands. Few rows are bound by the cache's bytes: a
     // second term (what the rounding left) costs nothing there. Many rows are bound by the products and
     // keep one term: half a step of relative error a weight, of both signs, in sums divided by the same
     // rounded weights' sum. An f32 output gets 24 bits from three terms (f16: 22 from two, and the rest).
-    c += constant("FEW_TERMS", st.out_dtype == SANIC_F32 ? 3 : 2) + constant("MANY_TERMS", st.out_dtype == SANIC_F32 ? 3 : 1);
+    c += number("FEW_TERMS", st.out_dtype == SANIC_F32 ? 3 : 2) + number("MANY_TERMS", st.out_dtype == SANIC_F32 ? 3 : 1);
     L.kernel_kind = "operator:paged_attn[mfma]";
     L.source = std::string(kPrelude) + kElement + c + kMfma;
     ln.grid = dim3((unsigned)(NKV * (few + live + std::max(tiles, PSPLIT))));

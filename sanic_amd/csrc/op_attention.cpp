@@ -116,9 +116,19 @@ struct Args { const unsigned short *q, *k, *v; const unsigned *tables, *starts, 
 constexpr bool HALF = DQ == 2;
 constexpr int CH = HD / 8, CG = (CH + 3) / 4;    // 16-byte chunks of a key's row, and 64-byte groups of them
 constexpr int DSTEP = CG, DT = HD / 16;          // products over 32 head dims; value tiles of 16 dims
-constexpr int LOADS = (TK / 16 * CG + 3) / 4;    // 16-byte loads a lane for a tile's keys, and its values
-constexpr int TILE = LOADS * 4 * 512;            // elements of a staged tile, surplus loads included
-constexpr int KG = TK / 16, DH = 4 / KG, DTH = DH == 1 ? DT : (DT + 3) / 4 * 2;
+// tiles of TK keys in a ring of ST
+template <int TK_, int ST_> struct Ring {
+  static constexpr int TK = TK_, ST = ST_;
+  static constexpr int LOADS = (TK / 16 * CG + 3) / 4;   // 16-byte loads a lane for a tile's keys, and its values
+  static constexpr int TILE = LOADS * 4 * 512;           // elements of a staged tile, surplus loads included
+  static constexpr int SIZE = ST * 2 * TILE;
+  static __device__ __forceinline__ int at(int buf, int value) { return (buf * 2 + value) * TILE; }
+};
+typedef Ring<FEW_TK, FEW_ST> Few;
+typedef Ring<MANY_TK, MANY_ST> Many;
+constexpr int KG = FEW_TK / 16, DH = 4 / KG, DTH = DH == 1 ? DT : (DT + 3) / 4 * 2;   // few rows: key groups, dim parts
+static_assert(KG * 32 * HD * 4 <= Few::SIZE * 2 && 256 * 24 <= Few::SIZE * 2);
+constexpr int RING = Few::SIZE > Many::SIZE || !PITEMS ? Few::SIZE : Many::SIZE;
 constexpr int MBS = M * BS;                      // positions a block table can hold
 constexpr float NEG_INF = -__builtin_huge_valf();
 
@@ -160,7 +170,7 @@ __device__ __forceinline__ int clamp_pos(long long p) { return p < 0 ? 0 : p > M
 
 // (one object: with several, the compiler waits for every load into LDS before any read of it)
 __shared__ struct {
-  __attribute__((aligned(1024))) unsigned short ring[STAGES][2][TILE];
+  __attribute__((aligned(1024))) unsigned short ring[RING];
   unsigned pages[PAGES];
   unsigned long long odd_keys;
   int holes, last_arrival;
@@ -173,7 +183,7 @@ struct Item {
 };
 struct Req {
   long long start, past;
-  int rows, tiles, kt;
+  int rows, tiles, kt;   // packed rows; workgroups of PR of them (0: few rows, D below); key tiles
 };
 __device__ __forceinline__ Req request(const Args& a, int b) {
   Req q{0, 0, 0, 0, 0};
@@ -184,7 +194,7 @@ __device__ __forceinline__ Req request(const Args& a, int b) {
   q.rows = (int)(e - s) * REP;
   q.tiles = q.rows <= DR ? 0 : (q.rows + PR - 1) / PR;
   const int hi = clamp_pos(q.past + (e - s)), lo = W ? clamp_pos(q.past + 1 - W) : 0;
-  const int kt = (hi + TK - 1) / TK - lo / TK;
+  const int tk = q.tiles ? MANY_TK : FEW_TK, kt = (hi + tk - 1) / tk - lo / tk;
   q.kt = kt > 1 ? kt : 1;
   return q;
 }
@@ -199,73 +209,70 @@ __device__ __forceinline__ int scan64(int v) {  // inclusive, over the wave
   }
   return v;
 }
-// Every wave of every workgroup computes the same numbers in the same order. P: requests of more than
-// DR rows, D: the others.
-__device__ __forceinline__ bool find_item(const Args& a, int it, Item& o) {
+__device__ __forceinline__ int many_splits(int kt, int part) {
+  const int s = (kt + part - 1) / part;
+  return s < MOST ? s : MOST;
+}
+// What every wave of every workgroup computes alike from the lengths. Few-row requests' key tiles, one
+// request behind the other, are cut into equal runs of `run` tiles, one a workgroup; many-row tiles are
+// split into parts of `part` key tiles each.
+struct Plan {
+  int run, part, items, stride;    // items: of the many-row requests; stride: rows of a few-row partial
+};
+__device__ __forceinline__ Plan make_plan(const Args& a, Req& q) {
   const int lane = threadIdx.x & 63;
-  float ud = 0, rd = 0, urd = 0, up = 0, tp = 0;
-  int items = 0;
-  Req q;
+  float ud = 0, umax = 0, rmax = 0, up = 0, tp = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
     q = request(a, b0 + lane);
-    const bool d = q.tiles == 0;
-    ud += d ? q.kt : 0, rd += d ? q.rows : 0, urd += d ? (float)q.rows * q.kt : 0;
-    up += (float)q.tiles * q.kt, tp += q.tiles;
+    if (q.tiles == 0) {
+      ud += q.kt;
+      umax = __builtin_fmaxf(umax, q.kt), rmax = __builtin_fmaxf(rmax, q.rows);
+    } else {
+      up += (float)q.tiles * q.kt, tp += q.tiles;
+    }
   }
-  ud = sanic_wave_sum(ud), rd = sanic_wave_sum(rd), urd = sanic_wave_sum(urd);
-  if (PITEMS) up = sanic_wave_sum(up), tp = sanic_wave_sum(tp);
-  // split lengths in key tiles: items = Σ ⌈kt / length⌉ ≤ Σ kt / length + requests
-  const float never = 1e9f;
-  float ld = ud / DTARGET, lp = never;
-  const float room = (float)DROWS - rd - 1.0f;
-  if (room < rd) ld = never;
-  else ld = __builtin_fmaxf(ld, urd / room);
-  if (PITEMS && 2.0f * tp <= (float)PSPLIT) lp = up / ((float)PSPLIT - tp - 1.0f);
-  // (the sums are f32: 1.001 covers their roundings where a bound hangs on them)
-  const int len_d = __builtin_amdgcn_readfirstlane((int)__builtin_fmaxf(1.0f, __builtin_ceilf(__builtin_fminf(ld * 1.001f, never))));
-  const int len_p = __builtin_amdgcn_readfirstlane((int)__builtin_fmaxf(1.0f, __builtin_ceilf(__builtin_fminf(lp * 1.001f, never))));
-  // the many-row items first: they take longest
+  ud = sanic_wave_sum(ud), umax = sanic_wave_max(umax), rmax = sanic_wave_max(rmax);
+  Plan p;
+  p.stride = __builtin_amdgcn_readfirstlane((int)rmax);
+  // as many workgroups as run at once, or as their partials (two of `stride` rows each) have room, or as
+  // one request's parts may be for the workgroup that adds them (about MOST)
+  float groups = FEW_GROUPS;
+  if (rmax > 0.0f) groups = __builtin_fminf(groups, __builtin_floorf((float)DROWS / (2.0f * rmax)));
+  const float run = __builtin_fmaxf(ud / groups, umax / (float)MOST);
+  // (the sums are f32: 1.001 covers their roundings)
+  p.run = __builtin_amdgcn_readfirstlane((int)__builtin_fmaxf(1.0f, __builtin_ceilf(run * 1.001f)));
+  p.part = 1 << 30, p.items = 0;
   if (PITEMS) {
-    int before_t = 0;
+    up = sanic_wave_sum(up), tp = sanic_wave_sum(tp);
+    if (2.0f * tp <= (float)PSPLIT)
+      p.part = __builtin_amdgcn_readfirstlane((int)__builtin_fmaxf(1.0f, __builtin_ceilf(up / ((float)PSPLIT - tp - 1.0f) * 1.001f)));
     for (int b0 = 0; b0 < B; b0 += 64) {
       if (B > 64) q = request(a, b0 + lane);
-      int splits = (q.kt + len_p - 1) / len_p;
-      if (splits > MEET / PR) splits = MEET / PR;
-      const int mine = q.tiles * splits, inc = scan64(mine), tinc = scan64(q.tiles);
-      const unsigned long long who = __ballot(mine > 0 && it >= inc - mine && it < inc);
-      if (who) {
-        const int l = __builtin_ctzll(who), x = it - pick(inc - mine, l), tiles = pick(q.tiles, l);
-        o.b = b0 + l, o.splits = pick(splits, l), o.rows = pick(q.rows, l);
-        o.tile = tiles - 1 - x / o.splits;     // the last rows see most
-        o.split = x % o.splits;
-        o.slot = (int)DROWS + (items + it - o.split) * (int)PR;
-        o.count = (int)B + before_t + pick(tinc, l) - tiles + o.tile;
-        o.start = pick(q.start, l), o.past = pick(q.past, l);
-        return true;
-      }
-      const int all = pick(inc, 63);
-      it -= all, items += all, before_t += pick(tinc, 63);
+      p.items += pick(scan64(q.tiles * many_splits(q.kt, p.part)), 63);
     }
   }
-  int before_r = 0;
+  return p;
+}
+// The many-row item `it`.
+__device__ __forceinline__ void find_many(const Args& a, const Plan& p, Req& q, int it, Item& o) {
+  const int lane = threadIdx.x & 63;
+  int before = 0, tiles_before = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
     if (B > 64) q = request(a, b0 + lane);
-    int splits = (q.kt + len_d - 1) / len_d;
-    if (q.rows && splits > MEET / q.rows) splits = MEET / q.rows;
-    const int mine = q.tiles == 0 && q.rows ? splits : 0, inc = scan64(mine), rinc = scan64(mine * q.rows);
+    const int splits = many_splits(q.kt, p.part), mine = q.tiles * splits, inc = before + scan64(mine), tinc = scan64(q.tiles);
     const unsigned long long who = __ballot(mine > 0 && it >= inc - mine && it < inc);
     if (who) {
-      const int l = __builtin_ctzll(who);
-      o.b = b0 + l, o.tile = -1, o.splits = pick(mine, l), o.rows = pick(q.rows, l);
-      o.split = it - pick(inc - mine, l);
-      o.slot = before_r + pick(rinc - mine * q.rows, l);
-      o.count = o.b;
+      const int l = __builtin_ctzll(who), x = it - pick(inc - mine, l), tiles = pick(q.tiles, l);
+      o.b = b0 + l, o.splits = pick(splits, l), o.rows = pick(q.rows, l);
+      o.tile = tiles - 1 - x / o.splits;     // the last rows see most
+      o.split = x % o.splits;
+      o.slot = DROWS + (it - o.split) * PR;
+      o.count = B + tiles_before + pick(tinc, l) - tiles + o.tile;
       o.start = pick(q.start, l), o.past = pick(q.past, l);
-      return true;
+      return;
     }
-    it -= pick(inc, 63), before_r += pick(rinc, 63);
+    before = pick(inc, 63), tiles_before += pick(tinc, 63);
   }
-  return false;
 }
 
 // ── tiles of keys and values ──────────────────────────────────────────────────────────────────────
@@ -287,27 +294,46 @@ struct Stream {
     }
     if (hole) lds.holes = 1;
   }
-  __device__ __forceinline__ bool covers(int t0) const { return t0 / BS >= base && (t0 + TK - 1) / BS < base + PAGES; }
-  __device__ __forceinline__ void fetch(int t0, int buf) const {
+  template <class R> __device__ __forceinline__ bool covers(int t0) const { return t0 / BS >= base && (t0 + R::TK - 1) / BS < base + PAGES; }
+  template <class R> __device__ __forceinline__ void fetch(int t0, int buf) const {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = lane >> 2, c = (lane & 3) ^ (row >> 1 & 3);
+    // 16 rows of one page: its address is the wave's, a lane's part of it the same in every tile
+    unsigned page_of[R::LOADS];
     #pragma unroll
-    for (int u = 0; u < LOADS; u++) {
-      const int n = u * 4 + wave;
-      int group = n / CG, chunk = n % CG * 4 + c;
-      if (TK / 16 * CG % 4 && group >= TK / 16) group = TK / 16 - 1;
-      if (CH % 4 && chunk >= CH) chunk = CH - 1;    // (the query is 0 there)
-      const int key = t0 + group * 16 + row;
-      const unsigned page = lds.pages[key / BS - base];
-      const long long pg = page < NB ? page : 0, in = key % BS;    // a page that is none is read as block 0 and masked
-      const unsigned short* kp = k + (pg * K0 + in * K2 + chunk * 8);
-      const unsigned short* vp = v + (pg * V0 + in * V2 + chunk * 8);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)kp, (__attribute__((address_space(3))) void*)&lds.ring[buf][0][n * 512], 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vp, (__attribute__((address_space(3))) void*)&lds.ring[buf][1][n * 512], 16, 0, 0);
+    for (int u = 0; u < R::LOADS; u++) {
+      unsigned group = (unsigned)(u * 4 + wave) / CG;
+      if (R::TK / 16 * CG % 4 && group >= R::TK / 16) group = R::TK / 16 - 1;
+      if (BS % 16 == 0) page_of[u] = lds.pages[((unsigned)t0 + group * 16) / BS - base];
+    }
+    #pragma unroll
+    for (int u = 0; u < R::LOADS; u++) {
+      const unsigned n = u * 4 + wave;
+      unsigned group = n / CG;
+      const int cg = n % CG * 4;
+      int chunk = c;
+      if (R::TK / 16 * CG % 4 && group >= R::TK / 16) group = R::TK / 16 - 1;
+      if (CH % 4 && cg + c >= CH) chunk = CH - 1 - cg;    // (the query is 0 there)
+      const unsigned key = (unsigned)t0 + group * 16;
+      // a page that is none is read as block 0 and masked
+      const char *kp, *vp;
+      if (BS % 16 == 0) {
+        const unsigned page = __builtin_amdgcn_readfirstlane(page_of[u]);
+        const long long pg = page < NB ? page : 0, in = key % BS;
+        kp = (const char*)(k + (pg * K0 + in * K2 + cg * 8)) + (unsigned)(row * K2 + chunk * 8) * 2;
+        vp = (const char*)(v + (pg * V0 + in * V2 + cg * 8)) + (unsigned)(row * V2 + chunk * 8) * 2;
+      } else {
+        const unsigned page = lds.pages[(key + row) / BS - base];
+        const long long pg = page < NB ? page : 0, in = (key + row) % BS;
+        kp = (const char*)(k + (pg * K0 + in * K2 + (cg + chunk) * 8));
+        vp = (const char*)(v + (pg * V0 + in * V2 + (cg + chunk) * 8));
+      }
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)kp, (__attribute__((address_space(3))) void*)&lds.ring[R::at(buf, 0) + n * 512], 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vp, (__attribute__((address_space(3))) void*)&lds.ring[R::at(buf, 1) + n * 512], 16, 0, 0);
     }
   }
   // the keys of a tile that are in no block of the pool, a bit each
-  __device__ __forceinline__ unsigned long long missing(int t0) const {
+  template <int TK> __device__ __forceinline__ unsigned long long missing(int t0) const {
     unsigned long long out = 0;
     for (int p = t0 / BS; p <= (t0 + TK - 1) / BS; p++) {
       if (p < first_page || p > last_page || table[p] < NB) continue;
@@ -318,42 +344,53 @@ struct Stream {
   }
 };
 
+template <class R>
+__device__ __forceinline__ void need(Stream& st, int t0) {
+  if (st.covers<R>(t0)) return;
+  __syncthreads();
+  st.pages_from(t0 / BS);
+  __syncthreads();
+}
 // The first tiles under way. The query rows are waited for before them (behind the block table, which
 // is anyway): the compiler would otherwise wait for them, and so for every tile, inside the loop.
-template <int RT>
+template <class R, int RT>
 __device__ __forceinline__ void begin(Stream& st, int t_first, int t_last, s16x8 (&q)[RT][DSTEP]) {
   if (threadIdx.x == 0) lds.holes = 0;
   __syncthreads();
-  if (t_first < t_last) st.pages_from(t_first * TK / (int)BS);
+  if (t_first < t_last) st.pages_from(t_first * R::TK / BS);
   #pragma unroll
   for (int t = 0; t < RT; t++)
     #pragma unroll
     for (int d = 0; d < DSTEP; d++) asm volatile("" : "+v"(q[t][d]));
   __syncthreads();
-  if (t_first < t_last) st.fetch(t_first * TK, 0);
-  if (STAGES == 3 && t_first + 1 < t_last) {
-    if (!st.covers((t_first + 1) * TK)) {
-      __syncthreads();
-      st.pages_from((t_first + 1) * TK / (int)BS);
-      __syncthreads();
-    }
-    st.fetch((t_first + 1) * TK, 1);
+  #pragma unroll
+  for (int i = 0; i < R::ST - 1; i++) {
+    if (t_first + i >= t_last) break;
+    need<R>(st, (t_first + i) * R::TK);
+    st.fetch<R>((t_first + i) * R::TK, i);
   }
 }
-// tile `i` of the item has arrived in every wave's part; PD tiles are under way behind it
-__device__ __forceinline__ void arrived(int left) {
-  constexpr int PD = STAGES - 1;
-  if (PD == 2 && left > 0) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+// Tile t has arrived in every wave's part of it, and the tile before it is done with: the next tile
+// under way takes its place.
+template <class R>
+__device__ __forceinline__ void turn(Stream& st, int t, int t_last, int buf) {
+  const int left = t_last - 1 - t;      // tiles behind it that are under way: up to ST − 2
+  if (R::ST > 3 && left >= 2) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * 2 * R::LOADS) : "memory");
+  else if (R::ST > 2 && left >= 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * R::LOADS) : "memory");
   else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  if (t + R::ST - 1 < t_last) {
+    need<R>(st, (t + R::ST - 1) * R::TK);
+    st.fetch<R>((t + R::ST - 1) * R::TK, buf == 0 ? R::ST - 1 : buf - 1);
+  }
 }
 
-__device__ __forceinline__ s16x8 key_run(int buf, int group, int step, int l16, int lq) {
-  return *(const s16x8*)&lds.ring[buf][0][(group * CG + step) * 512 + in_block(l16, lq)];
+__device__ __forceinline__ s16x8 key_run(int tile, int group, int step, int l16, int lq) {
+  return *(const s16x8*)&lds.ring[tile + (group * CG + step) * 512 + in_block(l16, lq)];
 }
 // Transposed reads of 16 keys × 16 value dims: a lane gets 4 keys of one dim. A lane's place in a block
 // for an even tile of dims; for an odd one it is 32 bytes further or back (two chunks, swapped alike).
-__device__ __forceinline__ unsigned value_at(int buf, int l16, int lq) {
-  return (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned short*)&lds.ring[buf][1][in_block(lq * 4 + (l16 >> 2), l16 >> 1 & 1) + (l16 & 1) * 4];
+__device__ __forceinline__ unsigned value_at(int tile, int l16, int lq) {
+  return (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned short*)&lds.ring[tile + in_block(lq * 4 + (l16 >> 2), l16 >> 1 & 1) + (l16 & 1) * 4];
 }
 // (waited for in the same statement: the compiler takes an asm output as written at once)
 template <int I0, int I1>
@@ -412,11 +449,11 @@ __device__ __forceinline__ void weigh(f32x4 (&s)[N], bool full, unsigned long lo
 // where one that is seen is not finite, its key's bit is returned, and it is 0 in the tile: add_odd
 // adds it to the rows that see it. Rows [row0, row0 + rows) × chunks [c0, c0 + chunks), of which any row
 // sees [lo, hi) (rows counted from the tile's first key).
-__device__ __forceinline__ unsigned long long clean(int buf, unsigned long long holes, int row0, int rows, int c0, int chunks, int lo, int hi, int part, int parts) {
+__device__ __forceinline__ unsigned long long clean(int tile, unsigned long long holes, int row0, int rows, int c0, int chunks, int lo, int hi, int part, int parts) {
   unsigned long long odd = 0;
   for (int i = part; i < rows * chunks; i += parts) {
     const int row = row0 + i / chunks;
-    s16x8* p = (s16x8*)&lds.ring[buf][1][spot(row, c0 + i % chunks)];
+    s16x8* p = (s16x8*)&lds.ring[tile + spot(row, c0 + i % chunks)];
     s16x8 x = *p;
     const bool dead = row < lo || row >= hi || (holes >> row & 1);
     bool change = dead;
@@ -479,64 +516,56 @@ __device__ __forceinline__ void put4(o_t* p, f32x4 v) {
   }
 }
 // The splits of rows [row0, row0 + rows) meet: the last workgroup to arrive adds them in their order.
-// Split s of row r stands at slot + s·stride + r.
-__device__ __forceinline__ void meet(const Args& a, const Item& it, int g, int row0, int rows, int stride) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, splits = it.splits;
+// Split s of row r stands at slot + s·stride + r, of the first split (few rows) one place before.
+__device__ __forceinline__ void meet(const Args& a, const Item& it, int g, int row0, int rows, int stride, int first) {
+  const int tid = threadIdx.x, splits = it.splits;
+  auto place = [&](int s) { return it.slot + (s == 0 ? first : s * stride); };
   unsigned* cnt = a.counts + (long long)it.count * NKV + g;
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   if (tid == 0) {
-    lds.last_arrival = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)splits - 1u;
-    if (lds.last_arrival) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    if (ONE_XCD) {
+      lds.last_arrival = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)splits - 1u;
+    } else {
+      lds.last_arrival = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)splits - 1u;
+      if (lds.last_arrival) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    }
   }
   __syncthreads();
   if (!lds.last_arrival) return;
   if (tid == 0) *cnt = 0;      // the next launch's arrivals count from 0 again
-  // weights of the splits, 2^(m − max m) / Σ (0 for a row that saw nothing): splits·rows ≤ MEET of them
-  float* w = (float*)lds.ring;
-  static_assert(MEET * 4 <= sizeof(lds.ring) && 4096 <= sizeof(lds.ring));
-  for (int r = wave; r < rows; r += 4) {
-    float mx = NEG_INF, sum = 0.0f;
-    for (int s = lane; s < splits; s += 64) mx = __builtin_fmaxf(mx, part_stats(a, g, it.slot + s * stride + r)[0]);
-    mx = sanic_wave_max(mx);
-    const float ref = mx == NEG_INF ? 0.0f : mx;
-    for (int s = lane; s < splits; s += 64) {
-      const float* p = part_stats(a, g, it.slot + s * stride + r);
-      const float f = __builtin_amdgcn_exp2f(p[0] - ref);
-      w[s * rows + r] = f;
-      sum += p[1] * f;
-    }
-    sum = sanic_wave_sum(sum);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    for (int s = lane; s < splits; s += 64) w[s * rows + r] *= inv;
-  }
-  __syncthreads();
-  // a thread's sums: 4 value dims of a row; with few of them, teams take every teams-th split each and
-  // meet in LDS
-  const int units = rows * (int)(HD / 4), teams = units >= 256 ? 1 : 256 / units;
-  if (teams == 1) {
-    for (int u = tid; u < units; u += 256) {
-      const int r = u / (int)(HD / 4), d = u % (int)(HD / 4) * 4;
-      f32x4 acc = {0, 0, 0, 0};
+  // a thread's sums: 4 value dims of a row over the splits, statistics and sums loaded together; with few
+  // of them, teams take every teams-th split each and meet in LDS
+  const int units = rows * (HD / 4), teams = units >= 256 ? 1 : 256 / units;
+  const int team = teams == 1 ? 0 : tid / units;
+  for (int u = teams == 1 ? tid : tid % units; u < units; u += 256) {
+    const int r = u / (HD / 4), d = u % (HD / 4) * 4;
+    f32x4 acc = {0, 0, 0, 0};
+    float m = NEG_INF, l = 0.0f;
+    auto add = [&](float m2, float l2, f32x4 v) {
+      const float to = __builtin_fmaxf(m, m2), ref = to == NEG_INF ? 0.0f : to;   // (a split that saw nothing has weight 0)
+      const float f = __builtin_amdgcn_exp2f(m - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+      acc = acc * f + v * f2;
+      l = l * f + l2 * f2;
+      m = to;
+    };
+    if (team < teams) {
       #pragma unroll 4
-      for (int s = 0; s < splits; s++) acc += w[s * rows + r] * *(const f32x4*)(part_sums(a, g, it.slot + s * stride + r) + d);
-      put4(a.o + out_at(it, g, row0 + r) + d, acc);
+      for (int s = team; s < splits; s += teams) {
+        const f32x2 x = *(const f32x2*)part_stats(a, g, place(s) + r);
+        add(x[0], x[1], *(const f32x4*)(part_sums(a, g, place(s) + r) + d));
+      }
     }
-    return;
-  }
-  const int team = tid / units, u = tid % units, r = u / (int)(HD / 4), d = u % (int)(HD / 4) * 4;
-  f32x4 acc = {0, 0, 0, 0};
-  if (team < teams) {
-    #pragma unroll 8
-    for (int s = team; s < splits; s += teams) acc += w[s * rows + r] * *(const f32x4*)(part_sums(a, g, it.slot + s * stride + r) + d);
-  }
-  __syncthreads();
-  f32x4* mine = (f32x4*)lds.ring;
-  mine[tid] = acc;
-  __syncthreads();
-  if (team == 0) {
-    for (int k = 1; k < teams; k++) acc += mine[k * units + tid];
-    put4(a.o + out_at(it, g, row0 + r) + d, acc);
+    if (teams > 1) {
+      f32x4* sums = (f32x4*)lds.ring;
+      f32x2* stats = (f32x2*)(sums + 256);
+      sums[tid] = acc;
+      stats[tid] = (f32x2){m, l};
+      __syncthreads();
+      if (team != 0) break;
+      for (int k = 1; k < teams; k++) add(stats[k * units + tid][0], stats[k * units + tid][1], sums[k * units + tid]);
+    }
+    put4(a.o + out_at(it, g, row0 + r) + d, l == 0.0f ? (f32x4){0, 0, 0, 0} : acc / l);
   }
 }
 
@@ -560,7 +589,8 @@ __device__ __forceinline__ void few_values(unsigned at, s16x4 (&vt)[(DTH + 3) / 
 
 // ── few rows: the waves split the tile's keys ─────────────────────────────────────────────────────
 template <int RT>
-__device__ __forceinline__ void few_rows(const Args& a, const Item& it, int g, Stream& st, int t_first, int t_last, int lo_all, int hi_all, int full_lo, int full_hi) {
+__device__ __forceinline__ void few_rows(const Args& a, const Item& it, int stride, int g, Stream& st, int t_first, int t_last, int lo_all, int hi_all, int full_lo, int full_hi) {
+  constexpr int TK = FEW_TK;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
   const int kg = wave % KG, dh = wave / KG, dt0 = dh * DTH;
   s16x8 qf[RT][DSTEP];
@@ -582,28 +612,19 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int g, S
     #pragma unroll
     for (int d = 0; d < DTH; d++) o[t][d] = (f32x4){0, 0, 0, 0};
   }
-  begin(st, t_first, t_last, qf);
+  begin<Few>(st, t_first, t_last, qf);
   const short one = HALF ? (short)0x3C00 : (short)0x3F80;
   const s16x4 ones = {one, one, one, one};
   int buf = 0;
   for (int i = t_first; i < t_last; i++) {
     const int t0 = i * TK;
-    arrived(t_last - 1 - i);
-    if (i + STAGES - 1 < t_last) {
-      const int ahead = t0 + (STAGES - 1) * TK;
-      if (!st.covers(ahead)) {
-        __syncthreads();
-        st.pages_from(ahead / BS);
-        __syncthreads();
-      }
-      st.fetch(ahead, buf == 0 ? STAGES - 1 : buf - 1);
-    }
-    const unsigned long long holes = lds.holes ? st.missing(t0) : 0;
+    turn<Few>(st, i, t_last, buf);
+    const unsigned long long holes = lds.holes ? st.missing<TK>(t0) : 0;
     const bool full = t0 >= full_lo && t0 + TK <= full_hi && !holes;
     unsigned long long odd = 0;
     if (!full) {
       const int c0 = dt0 * 2, c1 = (dt0 + DTH) * 2 < CH ? (dt0 + DTH) * 2 : CH;
-      odd = clean(buf, holes, kg * 16, 16, c0, c1 - c0, lo_all - t0, hi_all - t0, lane, 64);
+      odd = clean(Few::at(buf, 1), holes, kg * 16, 16, c0, c1 - c0, lo_all - t0, hi_all - t0, lane, 64);
       for (int x = 1; x < 64; x <<= 1) odd |= __shfl_xor(odd, x);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
@@ -612,7 +633,7 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int g, S
     for (int t = 0; t < RT; t++) {
       f32x4 s[1] = {{0, 0, 0, 0}};
       #pragma unroll
-      for (int d = 0; d < DSTEP; d++) s[0] = mma32(key_run(buf, kg, d, l16, lq), qf[t][d], s[0]);
+      for (int d = 0; d < DSTEP; d++) s[0] = mma32(key_run(Few::at(buf, 0), kg, d, l16, lq), qf[t][d], s[0]);
       float factor;
       weigh<1>(s, full, holes, kg * 16 + lq * 4, lo[t] - t0, hi[t] - t0, m[t], factor);
       if (!__all(factor == 1.0f)) {
@@ -620,7 +641,7 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int g, S
         #pragma unroll
         for (int d = 0; d < DTH; d++) o[t][d] *= factor;
       }
-      if (t == 0) few_values<0>(value_at(buf, l16, lq) + (kg * CG + (dt0 >> 1)) * 1024, vt);
+      if (t == 0) few_values<0>(value_at(Few::at(buf, 1), l16, lq) + (kg * CG + (dt0 >> 1)) * 1024, vt);
       if (odd) add_odd<1, DTH>(st, odd, t0, kg * 16, s, o[t], dt0, lq);
       #pragma unroll
       for (int k = 0; k < FEW_TERMS; k++) {
@@ -630,7 +651,7 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int g, S
         for (int d = 0; d < DTH; d++) o[t][d] = mma16(vt[d], p, o[t][d]);
       }
     }
-    buf = buf == STAGES - 1 ? 0 : buf + 1;
+    buf = buf == Few::ST - 1 ? 0 : buf + 1;
   }
   // the key groups meet: maxima and sums, then the outputs, group after group
   __syncthreads();
@@ -662,20 +683,21 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int g, S
     if (it.splits == 1) {
       put4(a.o + out_at(it, g, row) + d, l == 0.0f ? (f32x4){0, 0, 0, 0} : v / l);
     } else {
-      *(f32x4*)(part_sums(a, g, it.slot + it.split * it.rows + row) + d) = v;
+      const int at = it.slot + (it.split ? it.split * 2 * stride : stride) + row;
+      *(f32x4*)(part_sums(a, g, at) + d) = v;
       if (d == 0) {
-        float* p = part_stats(a, g, it.slot + it.split * it.rows + row);
+        float* p = part_stats(a, g, at);
         p[0] = mx, p[1] = l;
       }
     }
   }
-  if (it.splits > 1) meet(a, it, g, 0, it.rows, it.rows);
+  if (it.splits > 1) meet(a, it, g, 0, it.rows, 2 * stride, stride);
 }
 
 // Oᵀ += Vᵀ·P over the tile, eight reads (all keys of two or four tiles of dims) at a time
 template <int D>
-__device__ __forceinline__ void many_values(unsigned at, const s16x8 (&p)[2][TK / 32][MANY_TERMS], f32x4 (&o)[2][DT]) {
-  constexpr int KS = TK / 32, G = 8 / (TK / 16);    // dim tiles a group
+__device__ __forceinline__ void many_values(unsigned at, const s16x8 (&p)[2][MANY_TK / 32][MANY_TERMS], f32x4 (&o)[2][DT]) {
+  constexpr int KS = MANY_TK / 32, G = 8 / (MANY_TK / 16);    // dim tiles a group
   constexpr int B0 = D / 2, B1 = D / 2 + 1 < CG ? D / 2 + 1 : D / 2;
   s16x4 r[8];
   if constexpr (KS == 2) tr_read8<B0 * 1024, (CG + B0) * 1024, (2 * CG + B0) * 1024, (3 * CG + B0) * 1024>(at, r);
@@ -699,9 +721,9 @@ __device__ __forceinline__ void many_values(unsigned at, const s16x8 (&p)[2][TK 
 
 // ── many rows: 32 a wave ──────────────────────────────────────────────────────────────────────────
 __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, Stream& st, int t_first, int t_last, int lo_all, int hi_all, int full_lo, int full_hi) {
-  constexpr int NK = TK / 16;
+  constexpr int TK = MANY_TK, NK = TK / 16;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
-  const int row0 = it.tile * (int)PR + wave * 32;
+  const int row0 = it.tile * PR + wave * 32;
   s16x8 qf[2][DSTEP];
   int lo[2], hi[2];
   #pragma unroll
@@ -726,29 +748,20 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
     #pragma unroll
     for (int d = 0; d < DT; d++) o[t][d] = (f32x4){0, 0, 0, 0};
   }
-  begin(st, t_first, t_last, qf);
+  begin<Many>(st, t_first, t_last, qf);
   const short one = HALF ? (short)0x3C00 : (short)0x3F80;
   const s16x8 ones = {one, one, one, one, one, one, one, one};
   int buf = 0;
   for (int i = t_first; i < t_last; i++) {
     const int t0 = i * TK;
-    arrived(t_last - 1 - i);
-    if (i + STAGES - 1 < t_last) {
-      const int ahead = t0 + (STAGES - 1) * TK;
-      if (!st.covers(ahead)) {
-        __syncthreads();
-        st.pages_from(ahead / BS);
-        __syncthreads();
-      }
-      st.fetch(ahead, buf == 0 ? STAGES - 1 : buf - 1);
-    }
-    const unsigned long long holes = lds.holes ? st.missing(t0) : 0;
+    turn<Many>(st, i, t_last, buf);
+    const unsigned long long holes = lds.holes ? st.missing<TK>(t0) : 0;
     unsigned long long odd = 0;
     if (!(t0 >= full_lo && t0 + TK <= full_hi) || holes) {
       // the tile is every wave's: cleaned by all, then used
       if (tid == 0) lds.odd_keys = 0;
       __syncthreads();
-      const unsigned long long mine = clean(buf, holes, 0, TK, 0, CH, lo_all - t0, hi_all - t0, tid, 256);
+      const unsigned long long mine = clean(Many::at(buf, 1), holes, 0, TK, 0, CH, lo_all - t0, hi_all - t0, tid, 256);
       if (mine) atomicOr(&lds.odd_keys, mine);
       __syncthreads();
       odd = lds.odd_keys;
@@ -761,7 +774,7 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
         s[0][kt] = (f32x4){0, 0, 0, 0}, s[1][kt] = (f32x4){0, 0, 0, 0};
         #pragma unroll
         for (int d = 0; d < DSTEP; d++) {
-          const s16x8 k = key_run(buf, kt, d, l16, lq);
+          const s16x8 k = key_run(Many::at(buf, 0), kt, d, l16, lq);
           s[0][kt] = mma32(k, qf[0][d], s[0][kt]);
           s[1][kt] = mma32(k, qf[1][d], s[1][kt]);
         }
@@ -786,11 +799,11 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
             sum[t] = mma32(ones, p[t][ks][k], sum[t]);
           }
       }
-      many_values<0>(value_at(buf, l16, lq), p, o);
+      many_values<0>(value_at(Many::at(buf, 1), l16, lq), p, o);
     }
-    buf = buf == STAGES - 1 ? 0 : buf + 1;
+    buf = buf == Many::ST - 1 ? 0 : buf + 1;
   }
-  const int tile_rows = it.rows - it.tile * (int)PR < PR ? it.rows - it.tile * (int)PR : (int)PR;
+  const int tile_rows = it.rows - it.tile * PR < PR ? it.rows - it.tile * PR : PR;
   #pragma unroll
   for (int t = 0; t < 2; t++) {
     const int r = wave * 32 + t * 16 + l16;
@@ -799,47 +812,82 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
     if (it.splits == 1) {
       const float f = l == 0.0f ? 0.0f : 1.0f / l;
       #pragma unroll
-      for (int d = 0; d < DT; d++) put4(a.o + out_at(it, g, it.tile * (int)PR + r) + d * 16 + lq * 4, o[t][d] * f);
+      for (int d = 0; d < DT; d++) put4(a.o + out_at(it, g, it.tile * PR + r) + d * 16 + lq * 4, o[t][d] * f);
     } else {
-      float* p = part_sums(a, g, it.slot + it.split * (int)PR + r);
+      float* p = part_sums(a, g, it.slot + it.split * PR + r);
       #pragma unroll
       for (int d = 0; d < DT; d++) *(f32x4*)(p + d * 16 + lq * 4) = o[t][d];
       if (lq == 0) {
-        float* x = part_stats(a, g, it.slot + it.split * (int)PR + r);
+        float* x = part_stats(a, g, it.slot + it.split * PR + r);
         x[0] = m[t], x[1] = l;
       }
     }
   }
-  if (it.splits > 1) meet(a, it, g, it.tile * (int)PR, tile_rows, (int)PR);
+  if (it.splits > 1) meet(a, it, g, it.tile * PR, tile_rows, PR, 0);
 }
 
-extern "C" __global__ void __launch_bounds__(256, OCC) sanic_paged_attn(Args a) {
-  const int g = (int)(blockIdx.x % NKV);
-  Item it;
-  if (!find_item(a, (int)(blockIdx.x / NKV), it)) return;
-  // the rows of this workgroup, and the keys that any and that all of them see
-  const int r0 = it.tile < 0 ? 0 : it.tile * (int)PR, r1 = it.tile < 0 || r0 + PR > it.rows ? it.rows : r0 + (int)PR;
+// Rows [r0, r1) of an item: what any and what all of them see, and the part of the key tiles.
+template <bool MANY>
+__device__ __forceinline__ void rows_of(const Args& a, const Item& it, int g, int r0, int r1, int t0, int t1, int stride) {
+  constexpr int TK = MANY ? MANY_TK : FEW_TK;
   const long long p0 = it.past + r0 / REP, p1 = it.past + (r1 - 1) / REP;
   const int hi_all = clamp_pos(p1 + 1), full_hi = clamp_pos(p0 + 1);
   const int lo_all = W ? clamp_pos(p0 + 1 - W) : 0, full_lo = W ? clamp_pos(p1 + 1 - W) : 0;
   const int k0 = lo_all / TK, k1 = lo_all < hi_all ? (hi_all + TK - 1) / TK : k0;
-  const int t_first = k0 + (int)((long long)(k1 - k0) * it.split / it.splits), t_last = k0 + (int)((long long)(k1 - k0) * (it.split + 1) / it.splits);
-  Stream st{a, a.tables + (long long)it.b * M, g, lo_all / (int)BS, (hi_all - 1) / (int)BS, 0, a.k + (KB + g * K1), a.v + (VB + g * V1)};
-  if (it.tile >= 0) {
-    if (PITEMS) many_rows(a, it, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
-  } else if (it.rows <= 16) {
-    few_rows<1>(a, it, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
+  Stream st{a, a.tables + (long long)it.b * M, g, lo_all / BS, (hi_all - 1) / BS, 0, a.k + (KB + g * K1), a.v + (VB + g * V1)};
+  if constexpr (MANY) {
+    const int t_first = k0 + (int)((long long)(k1 - k0) * it.split / it.splits), t_last = k0 + (int)((long long)(k1 - k0) * (it.split + 1) / it.splits);
+    many_rows(a, it, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
   } else {
-    few_rows<2>(a, it, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
+    const int t_first = k0 + t0 < k1 ? k0 + t0 : k1, t_last = k0 + t1 < k1 ? k0 + t1 : k1;
+    if (it.rows <= 16) few_rows<1>(a, it, stride, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
+    else few_rows<2>(a, it, stride, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
+  }
+}
+
+extern "C" __global__ void __launch_bounds__(256, OCC) sanic_paged_attn(Args a) {
+  const int g = (int)(blockIdx.x % NKV), lane = threadIdx.x & 63;
+  int w = (int)(blockIdx.x / NKV);
+  Req q;
+  const Plan p = make_plan(a, q);
+  Item it;
+  // the many-row items first: they take longest
+  if (PITEMS && w < p.items) {
+    find_many(a, p, q, w, it);
+    const int r0 = it.tile * PR, r1 = r0 + PR < it.rows ? r0 + PR : it.rows;
+    rows_of<true>(a, it, g, r0, r1, 0, 0, 0);
+    return;
+  }
+  // the requests in the w-th run of key tiles
+  w -= p.items;
+  const int r0 = w * p.run, r1 = r0 + p.run;
+  int before = 0;
+  for (int b0 = 0; b0 < B && before < r1; b0 += 64) {
+    if (B > 64) q = request(a, b0 + lane);
+    const int mine = q.tiles == 0 && q.rows ? q.kt : 0, inc = before + scan64(mine), exc = inc - mine;
+    unsigned long long who = __ballot(mine > 0 && inc > r0 && exc < r1);
+    while (who) {
+      const int l = __builtin_ctzll(who), from = pick(exc, l), to = pick(inc, l), w0 = from / p.run;
+      who &= who - 1;
+      it.b = b0 + l, it.tile = -1, it.rows = pick(q.rows, l);
+      it.splits = (to - 1) / p.run - w0 + 1, it.split = w - w0;
+      it.slot = w0 * 2 * p.stride;             // a request's first part is its workgroup's second partial
+      it.count = it.b;
+      it.start = pick(q.start, l), it.past = pick(q.past, l);
+      rows_of<false>(a, it, g, 0, it.rows, (r0 > from ? r0 : from) - from, (r1 < to ? r1 : to) - from, p.stride);
+      __syncthreads();
+    }
+    before = pick(inc, 63);
   }
 }
 )SRC";
 
 // The matrix-core kernel takes queries and caches of one 16-bit type whose rows are runs of a multiple
 // of 16 elements, in units of 16 bytes.
-static bool mfma_takes(const OperandView& q, const OperandView& k, const OperandView& v) {
+static bool mfma_takes(const OperandView& q, const OperandView& k, const OperandView& v, int64_t B, int64_t M) {
     const int64_t HD = q.extent[2];
     if (q.dtype != k.dtype || (q.dtype != SANIC_BF16 && q.dtype != SANIC_F16) || HD % 16 || HD > 256) return false;
+    if (B * (M * k.extent[2] / 32 + 1) >= int64_t(1) << 30) return false;     // key tiles are counted in 31 bits
     for (const OperandView* o : {&q, &k, &v}) {
         if (o->stride.back() != 1 || o->base % 8) return false;
         for (size_t j = 0; j + 1 < o->stride.size(); j++)
@@ -869,25 +917,26 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     Launch ln{"sanic_paged_attn", "", dim3((unsigned)((T * NH + 3) / 4)), dim3(256), 0, {}};
     for (int b : {q.buffer, k.buffer, v.buffer, tables.buffer, d->nodes[st.leaf[4]].buffer, d->nodes[st.leaf[5]].buffer, st.out_buffer})
         ln.args.push_back({Arg::BUF, b});
-    if (!mfma_takes(q, k, v) || !std::isfinite(scale)) {
+    if (!mfma_takes(q, k, v, B, M) || !std::isfinite(scale)) {
         L.kernel_kind = "operator:paged_attn[plain]";
         L.source = std::string(kPrelude) + kElement + c + kPlain;
         L.launches.push_back(ln);
         return L;
     }
-    // tiles: three of up to 8 KB for the keys and as much for the values leave three workgroups a CU
-    const int64_t TK = HD <= 64 ? 64 : 32, STAGES = HD <= 128 ? 3 : 2, OCC = HD <= 64 ? 3 : HD <= 192 ? 2 : 1;
-    const int64_t PR = 128, DR = 32, MEET = 4096;
+    const int64_t FEW_TK = HD <= 64 ? 64 : 32, FEW_ST = HD <= 64 ? 3 : HD <= 128 ? 4 : 2;
+    const int64_t MANY_TK = HD <= 128 ? 64 : 32, MANY_ST = HD <= 64 ? 3 : 2, OCC = HD <= 64 ? 3 : HD <= 192 ? 2 : 1;
+    const int64_t PR = 128, DR = 32, MOST = 256;
     const int64_t slots = 256 * OCC;
-    // items a key head: twice the workgroups that run at once
-    const int64_t live = std::min(B, T), few = std::max<int64_t>(1, 2 * slots / NKV);
-    const int64_t budget = (lean_scratch() ? int64_t(1) << 20 : int64_t(10) << 20) / (NKV * (HD + 2) * 4);
-    const int64_t DROWS = std::min((few + live) * std::min(DR, T * REP), budget);
+    const int64_t live = std::min(B, T), groups = std::max<int64_t>(1, slots / NKV);
+    const int64_t budget = (lean_scratch() ? int64_t(1) << 20 : int64_t(12) << 20) / (NKV * (HD + 2) * 4);
+    const int64_t DROWS = std::min(2 * groups * std::min(DR, T * REP), std::max(budget, 2 * DR));
     const int64_t tiles = T * REP > DR ? T * REP / PR + std::min(live, T * REP / (DR + 1)) : 0;
     const int64_t PSPLIT = tiles ? std::min(2 * slots / NKV, budget / PR) : 0;
     const int64_t SLOTS = DROWS + PSPLIT * PR;
-    c += number("TK", TK) + number("STAGES", STAGES) + number("OCC", OCC) + number("PR", PR) + number("DR", DR) + number("MEET", MEET);
-    c += number("DTARGET", few) + number("DROWS", DROWS) + number("PITEMS", tiles > 0) + number("PSPLIT", PSPLIT) + number("SLOTS", SLOTS);
+    c += number("FEW_TK", FEW_TK) + number("FEW_ST", FEW_ST) + number("MANY_TK", MANY_TK) + number("MANY_ST", MANY_ST);
+    c += number("OCC", OCC) + number("PR", PR) + number("DR", DR) + number("MOST", MOST);
+    c += number("FEW_GROUPS", groups) + number("DROWS", DROWS) + number("PITEMS", tiles > 0) + number("PSPLIT", PSPLIT) + number("SLOTS", SLOTS);
+    c += number("ONE_XCD", xcd_local_enabled() && NKV % 8 == 0);
     c += number("PAGES", 512) + number("FLIP", scale < 0) + "constexpr float C2 = " + flit(std::fabs(scale) * 1.4426950408889634) + ";\n";
     // Weights take the 16 bits of the matrix cores' operands. Few rows are bound by the cache's bytes: a
     // second term (what the rounding left) costs nothing there. Many rows are bound by the products and
@@ -896,7 +945,7 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     c += number("FEW_TERMS", st.out_dtype == SANIC_F32 ? 3 : 2) + number("MANY_TERMS", st.out_dtype == SANIC_F32 ? 3 : 1);
     L.kernel_kind = "operator:paged_attn[mfma]";
     L.source = std::string(kPrelude) + kElement + c + kMfma;
-    ln.grid = dim3((unsigned)(NKV * (few + live + std::max(tiles, PSPLIT))));
+    ln.grid = dim3((unsigned)(NKV * (groups + std::max(tiles, PSPLIT))));
     ln.args.push_back({Arg::SCRATCH, shared_scratch(scratch, NKV * SLOTS * (HD + 2) * 4)});
     ln.args.push_back({Arg::COUNTERS, shared_counters((B + PSPLIT / 2 + 1) * NKV)});
     L.launches.push_back(ln);

@@ -245,7 +245,8 @@ __device__ __forceinline__ Plan make_plan(const Args& a, Req& q) {
   if (PITEMS) {
     up = sanic_wave_sum(up), tp = sanic_wave_sum(tp);
     if (2.0f * tp <= (float)PSPLIT)
-      p.part = __builtin_amdgcn_readfirstlane((int)__builtin_fmaxf(1.0f, __builtin_ceilf(up / ((float)PSPLIT - tp - 1.0f) * 1.001f)));
+      // (no room beside one tile: as good as never)
+      p.part = __builtin_amdgcn_readfirstlane((int)__builtin_fminf(1e9f, __builtin_fmaxf(1.0f, __builtin_ceilf(up / ((float)PSPLIT - tp - 1.0f) * 1.001f))));
     for (int b0 = 0; b0 < B; b0 += 64) {
       if (B > 64) q = request(a, b0 + lane);
       p.items += pick(scan64(q.tiles * many_splits(q.kt, p.part)), 63);
@@ -520,7 +521,7 @@ __device__ __forceinline__ void put4(o_t* p, f32x4 v) {
 __device__ __forceinline__ void meet(const Args& a, const Item& it, int g, int row0, int rows, int stride, int first) {
   const int tid = threadIdx.x, splits = it.splits;
   auto place = [&](int s) { return it.slot + (s == 0 ? first : s * stride); };
-  unsigned* cnt = a.counts + (long long)it.count * NKV + g;
+  unsigned* cnt = a.counts + ((long long)g * COUNTS + it.count * CPAD);
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   if (tid == 0) {
@@ -888,6 +889,7 @@ static bool mfma_takes(const OperandView& q, const OperandView& k, const Operand
     const int64_t HD = q.extent[2];
     if (q.dtype != k.dtype || (q.dtype != SANIC_BF16 && q.dtype != SANIC_F16) || HD % 16 || HD > 256) return false;
     if (B * (M * k.extent[2] / 32 + 1) >= int64_t(1) << 30) return false;     // key tiles are counted in 31 bits
+    if (k.stride[2] >= int64_t(1) << 26 || v.stride[2] >= int64_t(1) << 26) return false;   // 16 rows of a page within 32 bits
     for (const OperandView* o : {&q, &k, &v}) {
         if (o->stride.back() != 1 || o->base % 8) return false;
         for (size_t j = 0; j + 1 < o->stride.size(); j++)
@@ -936,6 +938,12 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     c += number("FEW_TK", FEW_TK) + number("FEW_ST", FEW_ST) + number("MANY_TK", MANY_TK) + number("MANY_ST", MANY_ST);
     c += number("OCC", OCC) + number("PR", PR) + number("DR", DR) + number("MOST", MOST);
     c += number("FEW_GROUPS", groups) + number("DROWS", DROWS) + number("PITEMS", tiles > 0) + number("PSPLIT", PSPLIT) + number("SLOTS", SLOTS);
+    // arrival counters: a head's on lines of their own (a line that several XCDs count on goes back and
+    // forth between them), each on one while the 16384 static ones last
+    int64_t cpad = 32;
+    auto counts = [&] { return ((B + PSPLIT / 2 + 1) * cpad + 31) / 32 * 32; };
+    while (cpad > 1 && counts() * NKV > 16384) cpad /= 2;
+    c += number("COUNTS", counts()) + number("CPAD", cpad);
     c += number("ONE_XCD", xcd_local_enabled() && NKV % 8 == 0);
     c += number("PAGES", 512) + number("FLIP", scale < 0) + "constexpr float C2 = " + flit(std::fabs(scale) * 1.4426950408889634) + ";\n";
     // Weights take the 16 bits of the matrix cores' operands. Few rows are bound by the cache's bytes: a
@@ -947,7 +955,7 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     L.source = std::string(kPrelude) + kElement + c + kMfma;
     ln.grid = dim3((unsigned)(NKV * (groups + std::max(tiles, PSPLIT))));
     ln.args.push_back({Arg::SCRATCH, shared_scratch(scratch, NKV * SLOTS * (HD + 2) * 4)});
-    ln.args.push_back({Arg::COUNTERS, shared_counters((B + PSPLIT / 2 + 1) * NKV)});
+    ln.args.push_back({Arg::COUNTERS, shared_counters(counts() * NKV)});
     L.launches.push_back(ln);
     return L;
 }

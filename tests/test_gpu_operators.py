@@ -335,6 +335,7 @@ ATTN = {
     "many_short": dict(past=[3 * i % 41 for i in range(90)], new=[1 + (i % 7 == 0) for i in range(90)], NKV=2, rep=4, HD=64, BS=16),
     "long_and_short": dict(past=[9000] + [30] * 9, new=[1] * 10, NKV=1, rep=4, HD=64, BS=16),
     "long_chunk": dict(past=[3000], new=[40], NKV=1, rep=4, HD=64, BS=16),
+    "room_for_two_parts": dict(past=[100], new=[40], NKV=32, rep=1, HD=256, BS=16),
     "long_drafts_128": dict(past=[4000, 10], new=[4, 4], NKV=1, rep=8, HD=128, BS=16),
 }
 
@@ -505,6 +506,15 @@ def test_verify_all_and_none_accepted(dev):
     q[np.arange(T - 1), vals["tokens"][1:]] = 1.0
     assert check_verify(dev, dict(vals, q=q, u=np.full(T, 0.99)), ir.F32, ir.F32)[1] == [0, 0]
     assert check_verify(dev, dict(vals, u=np.ones(T)), ir.F32, ir.F32)[1] == [0, 0]
+
+
+def test_verify_nothing_left_over_a_large_vocabulary(dev):
+    """Refused with p == q: the token is drawn from p, also where many workgroups share the row."""
+    g = np.random.default_rng(8)
+    V, T = 50021, 4
+    p = stored(_softmax(g.standard_normal((T, V))), ir.F32)
+    vals = {"p": p, "q": p, "tokens": g.integers(0, V, T), "starts": [0, 2, 4], "u": np.ones(T), "draw": [0.37, 0.81]}
+    assert check_verify(dev, vals, ir.F32, ir.F32)[1] == [0, 0]
 
 
 @pytest.mark.parametrize("drafts", [63, 64, 65, 130])

@@ -233,11 +233,13 @@ __device__ __forceinline__ Plan make_plan(const Args& a, Req& q) {
   }
   ud = sanic_wave_sum(ud), umax = sanic_wave_max(umax), rmax = sanic_wave_max(rmax);
   Plan p;
-  p.stride = __builtin_amdgcn_readfirstlane((int)rmax);
+  // whole 128-byte lines of statistics and sums: the workgroup that adds one request's parts reads no line
+  // that holds another's, which its CU's L1 would keep as it was and a later join there would read
+  p.stride = (__builtin_amdgcn_readfirstlane((int)rmax) + LINE - 1) / LINE * LINE;
   // as many workgroups as run at once, or as their partials (two of `stride` rows each) have room, or as
   // one request's parts may be for the workgroup that adds them (about MOST)
   float groups = FEW_GROUPS;
-  if (rmax > 0.0f) groups = __builtin_fminf(groups, __builtin_floorf((float)DROWS / (2.0f * rmax)));
+  if (p.stride > 0) groups = __builtin_fminf(groups, __builtin_floorf((float)DROWS / (2.0f * (float)p.stride)));
   const float run = __builtin_fmaxf(ud / groups, umax / (float)MOST);
   // (the sums are f32: 1.001 covers their roundings)
   p.run = __builtin_amdgcn_readfirstlane((int)__builtin_fmaxf(1.0f, __builtin_ceilf(run * 1.001f)));
@@ -927,16 +929,16 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     }
     const int64_t FEW_TK = HD <= 64 ? 64 : 32, FEW_ST = HD <= 64 ? 3 : HD <= 128 ? 4 : 2;
     const int64_t MANY_TK = HD <= 128 ? 64 : 32, MANY_ST = HD <= 64 ? 3 : 2, OCC = HD <= 64 ? 3 : HD <= 192 ? 2 : 1;
-    const int64_t PR = 128, DR = 32, MOST = 256;
+    const int64_t PR = 128, DR = 32, MOST = 256, LINE = 16;
     const int64_t slots = 256 * OCC;
     const int64_t live = std::min(B, T), groups = std::max<int64_t>(1, slots / NKV);
     const int64_t budget = (lean_scratch() ? int64_t(1) << 20 : int64_t(12) << 20) / (NKV * (HD + 2) * 4);
-    const int64_t DROWS = std::min(2 * groups * std::min(DR, T * REP), std::max(budget, 2 * DR));
+    const int64_t DROWS = std::min(2 * groups * std::min(DR, (T * REP + LINE - 1) / LINE * LINE), std::max(budget, 2 * DR)) / LINE * LINE;
     const int64_t tiles = T * REP > DR ? T * REP / PR + std::min(live, T * REP / (DR + 1)) : 0;
     const int64_t PSPLIT = tiles ? std::min(2 * slots / NKV, budget / PR) : 0;
     const int64_t SLOTS = DROWS + PSPLIT * PR;
     c += number("FEW_TK", FEW_TK) + number("FEW_ST", FEW_ST) + number("MANY_TK", MANY_TK) + number("MANY_ST", MANY_ST);
-    c += number("OCC", OCC) + number("PR", PR) + number("DR", DR) + number("MOST", MOST);
+    c += number("OCC", OCC) + number("PR", PR) + number("DR", DR) + number("MOST", MOST) + number("LINE", LINE);
     c += number("FEW_GROUPS", groups) + number("DROWS", DROWS) + number("PITEMS", tiles > 0) + number("PSPLIT", PSPLIT) + number("SLOTS", SLOTS);
     // arrival counters: a head's on lines of their own (a line that several XCDs count on goes back and
     // forth between them), each on one while the 16384 static ones last

@@ -921,12 +921,6 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     Launch ln{"sanic_paged_attn", "", dim3((unsigned)((T * NH + 3) / 4)), dim3(256), 0, {}};
     for (int b : {q.buffer, k.buffer, v.buffer, tables.buffer, d->nodes[st.leaf[4]].buffer, d->nodes[st.leaf[5]].buffer, st.out_buffer})
         ln.args.push_back({Arg::BUF, b});
-    if (!mfma_takes(q, k, v, B, M) || !std::isfinite(scale)) {
-        L.kernel_kind = "operator:paged_attn[plain]";
-        L.source = std::string(kPrelude) + kElement + c + kPlain;
-        L.launches.push_back(ln);
-        return L;
-    }
     const int64_t FEW_TK = HD <= 64 ? 64 : 32, FEW_ST = HD <= 64 ? 3 : HD <= 128 ? 4 : 2;
     const int64_t MANY_TK = HD <= 128 ? 64 : 32, MANY_ST = HD <= 64 ? 3 : 2, OCC = HD <= 64 ? 3 : HD <= 192 ? 2 : 1;
     const int64_t PR = 128, DR = 32, MOST = 256, LINE = 16;
@@ -936,7 +930,16 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     const int64_t DROWS = std::min(2 * groups * std::min(DR, (T * REP + LINE - 1) / LINE * LINE), std::max(budget, 2 * DR)) / LINE * LINE;
     const int64_t tiles = T * REP > DR ? T * REP / PR + std::min(live, T * REP / (DR + 1)) : 0;
     const int64_t PSPLIT = tiles ? std::min(2 * slots / NKV, budget / PR) : 0;
-    const int64_t SLOTS = DROWS + PSPLIT * PR;
+    const int64_t SLOTS = DROWS + PSPLIT * PR, per_head = groups + std::max(tiles, PSPLIT);
+    // a workgroup's first key tile, its number times the run's length, stays within 31 bits
+    const int64_t most = M * BS / FEW_TK + 2, room = std::max<int64_t>(1, std::min(groups, DROWS / (2 * DR)));
+    const double run = 1.002 * std::max((double)B * most / room, (double)most / MOST) + 2;
+    if (!mfma_takes(q, k, v, B, M) || !std::isfinite(scale) || (per_head + 1) * run >= 2147483648.0) {
+        L.kernel_kind = "operator:paged_attn[plain]";
+        L.source = std::string(kPrelude) + kElement + c + kPlain;
+        L.launches.push_back(ln);
+        return L;
+    }
     c += number("FEW_TK", FEW_TK) + number("FEW_ST", FEW_ST) + number("MANY_TK", MANY_TK) + number("MANY_ST", MANY_ST);
     c += number("OCC", OCC) + number("PR", PR) + number("DR", DR) + number("MOST", MOST) + number("LINE", LINE);
     c += number("FEW_GROUPS", groups) + number("DROWS", DROWS) + number("PITEMS", tiles > 0) + number("PSPLIT", PSPLIT) + number("SLOTS", SLOTS);
@@ -955,7 +958,7 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     c += number("FEW_TERMS", st.out_dtype == SANIC_F32 ? 3 : 2) + number("MANY_TERMS", st.out_dtype == SANIC_F32 ? 3 : 1);
     L.kernel_kind = "operator:paged_attn[mfma]";
     L.source = std::string(kPrelude) + kElement + c + kMfma;
-    ln.grid = dim3((unsigned)(NKV * (groups + std::max(tiles, PSPLIT))));
+    ln.grid = dim3((unsigned)(NKV * per_head));
     ln.args.push_back({Arg::SCRATCH, shared_scratch(scratch, NKV * SLOTS * (HD + 2) * 4)});
     ln.args.push_back({Arg::COUNTERS, shared_counters(counts() * NKV)});
     L.launches.push_back(ln);

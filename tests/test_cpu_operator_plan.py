@@ -1,11 +1,12 @@
 """How the matrix-core attention over a paged cache divides its work, modelled on the CPU with the
 constants of the emitted source: every partial within its area and on 128-byte lines of its own, every
-workgroup in the grid, every arrival counter in its range."""
+workgroup in the grid, every arrival counter in its range, no index past 31 bits."""
 import math
 import random
 import re
 
 import numpy as np
+import pytest
 
 from sanic_amd import ir
 from sanic_amd.program import Program
@@ -90,7 +91,7 @@ def check(c, new, past):
     rows = c["T"] * c["REP"]
     bound = rows // c["PR"] + min(c["B"], c["T"], rows // (c["DR"] + 1)) if rows > c["DR"] else 0
     grid = c["FEW_GROUPS"] + max(bound, c["PSPLIT"])
-    assert items + top + 1 <= grid
+    assert items + top + 1 <= grid and (grid + 1) * run < 1 << 31
     return parts_few, len(spans) - parts_few
 
 
@@ -127,3 +128,10 @@ def test_random_batches():
         parts += sum(check(c, new, past))
         tried += 1
     assert parts > 1000
+
+@pytest.mark.parametrize("T,B,M,mfma", [(64, 64, 1 << 15, True), (1 << 16, 8192, 1 << 10, True), (1 << 22, 8192, 1 << 12, False)])
+def test_runs_are_counted_in_31_bits(T, B, M, mfma):
+    """A workgroup's first key tile is its number times the run's length: what could pass 31 bits takes
+    the kernel without runs."""
+    kind, c = emitted(T, 1, 16, 64, 64, B, M)
+    assert (kind == "operator:paged_attn[mfma]") == mfma

@@ -12,7 +12,9 @@ namespace sanic {
 
 // One wave per (row, head), keys 64 at a time, one per lane for the scores and one value dim per lane
 // for the output; m, the sum and the output in f32 over one pass. For every type, head size and
-// layout.
+// layout. Bound by its f32 operations and by reading every key once a row: 16 to 70 times the
+// matrix-core kernel's time where both can run (a token of each of 64 requests 3848 us against 236, 4096
+// rows of a prompt behind 12288 tokens 82.9 ms against 1.16).
 static const char* kPlain = R"SRC(
 typedef sanic_elem<DQ>::T q_t;
 typedef sanic_elem<DC>::T kv_t;
@@ -89,10 +91,21 @@ extern "C" __global__ void __launch_bounds__(256) sanic_paged_attn(Args a) {
 // TK keys come straight from the pages into a ring of LDS buffers (16 bytes a lane, no register
 // staging), addressed through the item's part of the block table in LDS.
 //
-// Work is split over keys too: request lengths are known on the device alone, so every workgroup sums
-// the requests' key tiles and derives the same split length, such that the items fill the chip a few
-// times over and their partials fit the scratch; it then finds its own item in the prefix sums. The
-// parts of one row meet in the workgroup that arrives last, which adds them in split order.
+// Work is split over keys too. Request lengths are known on the device alone, so every workgroup sums
+// the requests' key tiles and derives the same plan. The few-row requests' tiles, one request behind
+// the other, are cut into as many equal runs as workgroups are resident: a run may end one request and
+// begin the next, and no workgroup has more than another (24 requests of 5 drafts: 55 us; an item a
+// workgroup, with the longest request's items last, 68). Many-row tiles are split into parts over the
+// keys. Either way the partials fit the scratch. The parts of one row meet in the workgroup that
+// arrives last, which adds them in split order. The arrivals are relaxed where a key head's workgroups
+// share an XCD, whose L2 they meet in (a release writes that L2 back: 103 us instead of 68).
+//
+// Bound by HBM for decoded tokens: 64 requests of 32/8 heads of 128, 1.2 GB of cache, 236 us, 5.1 TB/s
+// (a large copy: 5.2); 10 us for one request, a chain of dependent loads. Bound by the matrix cores for
+// a prompt: 4096 rows of 32/8 heads of 128 behind 12288 tokens, 1157 us, 831 TFLOP/s (a large product: 1235). What brought
+// it there from 2911 us: tiles as blocks of 1 KB whose reads differ by constant offsets, and eight
+// transposed reads to one wait (1795); page addresses in scalar registers (1157; the 64 requests 310 to
+// 236).
 //
 // Scores are computed transposed (Sᵀ = K·Qᵀ), so a lane owns one row's column: softmax statistics are
 // lane-local plus two lane swaps, and Sᵀ's layout is the B operand of Oᵀ = Vᵀ·P as it stands. Softmax
@@ -921,6 +934,13 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     Launch ln{"sanic_paged_attn", "", dim3((unsigned)((T * NH + 3) / 4)), dim3(256), 0, {}};
     for (int b : {q.buffer, k.buffer, v.buffer, tables.buffer, d->nodes[st.leaf[4]].buffer, d->nodes[st.leaf[5]].buffer, st.out_buffer})
         ln.args.push_back({Arg::BUF, b});
+    // Tiles and rings: what lets OCC workgroups share 160 KB of LDS and, at 256 threads, 512 / OCC
+    // registers. Heads of 64: tiles of 64 keys, 3 deep, 3 workgroups a CU (24 requests of 5 drafts 49.8
+    // us, a mixed batch 60.8; with the plan of that time 55.8 and 63.2 against 63.8 and 73.3 for tiles
+    // of 32 and 4 workgroups, 63.5 and 77.5 for 2 workgroups). Heads of 128: 2 workgroups, many rows in
+    // tiles of 64 in a ring of 2 (those 4096 rows 1660 us at that time; tiles of 32 in a ring of 3
+    // 1770). Few-row workgroups as many as are resident: 2/3 of them 63.9 us for the drafts, twice as
+    // many 68.7, against 55.8.
     const int64_t FEW_TK = HD <= 64 ? 64 : 32, FEW_ST = HD <= 64 ? 3 : HD <= 128 ? 4 : 2;
     const int64_t MANY_TK = HD <= 128 ? 64 : 32, MANY_ST = HD <= 64 ? 3 : 2, OCC = HD <= 64 ? 3 : HD <= 192 ? 2 : 1;
     const int64_t PR = 128, DR = 32, MOST = 256, LINE = 16;

@@ -9,6 +9,8 @@ namespace sanic {
 // One launch, no exchange between workgroups: each repeats the two prefix sums over the requests
 // (lengths cut at T, then the blocks wanted) in LDS and serves its share of the rows and of the new
 // blocks with a binary search in them. Bound by latency: lengths, scan, search, table entry, store.
+// 8 requests 3.8 us (a launch alone is most of it), 512 requests 5.7; the lengths are a few KB, so a
+// launch of its own for the sums would cost more than every workgroup's repeating them.
 static const char* kTables = R"SRC(
 struct Args { const unsigned *past, *fresh, *held, *free; unsigned *tables, *slots, *positions, *held_next, *starts; };
 
@@ -121,7 +123,8 @@ LoweredStage lower_block_tables(const sanic_program_desc* d, const sanic_stage& 
 
 // One thread per run of RUN elements of a row, K's and V's: with rows of a multiple of 8 elements and
 // strides to match, 16 to 32 bytes a load and 16 a store, else one element. Bound by HBM for a
-// prompt's rows and by the launch for a decode step's.
+// prompt's rows (4096 rows of 8 heads of 128, bf16: 33.6 MB in 6.4 us, 5.3 TB/s, a large copy 5.2) and
+// by the launch for a decode step's (8 rows: 3.5 us).
 static const char* kWrite = R"SRC(
 typedef sanic_elem<DS>::T src_t;
 typedef sanic_elem<DD>::T dst_t;

@@ -16,7 +16,9 @@ namespace sanic {
 // of 24, and with them the drawn index), and the last to arrive finds the run that the draw falls into
 // from the runs' sums and reads that run again. All of a request's workgroups are on one XCD (block
 // index mod 8) where the device places blocks so, and meet through its L2. Bound by HBM for a batch and
-// by the chain of dependent loads (starts, tokens, tests, row, sums, run) for one request.
+// by the chain of dependent loads (starts, tokens, tests, row, sums, run) for one request: one request
+// of 128256 entries 12.4 us, 64 of them 22.5 (floor 12.7), 200 of 32003 without q 18.8; with one workgroup a
+// request 213, 244 and 24.7.
 static const char* kVerify = R"SRC(
 typedef sanic_elem<DP>::T p_t;
 typedef sanic_elem<DQ>::T q_t;

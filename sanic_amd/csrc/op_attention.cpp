@@ -904,7 +904,8 @@ static bool mfma_takes(const OperandView& q, const OperandView& k, const Operand
     const int64_t HD = q.extent[2];
     if (q.dtype != k.dtype || (q.dtype != SANIC_BF16 && q.dtype != SANIC_F16) || HD % 16 || HD > 256) return false;
     if (B * (M * k.extent[2] / 32 + 1) >= int64_t(1) << 30) return false;     // key tiles are counted in 31 bits
-    if (k.stride[2] >= int64_t(1) << 26 || v.stride[2] >= int64_t(1) << 26) return false;   // 16 rows of a page within 32 bits
+    for (const OperandView* o : {&k, &v})
+        if (o->stride[2] < 0 || o->stride[2] >= int64_t(1) << 26) return false;   // 16 rows of a page: an unsigned offset of 32 bits
     for (const OperandView* o : {&q, &k, &v}) {
         if (o->stride.back() != 1 || o->base % 8) return false;
         for (size_t j = 0; j + 1 < o->stride.size(); j++)

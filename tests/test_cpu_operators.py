@@ -116,6 +116,15 @@ REFUSED = {
 }
 
 
+@pytest.mark.parametrize("which", ["kc", "vc"])
+def test_blocks_read_backwards_take_the_plain_kernel(which):
+    """The matrix-core kernel adds a row's place in its block as an unsigned offset."""
+    p = attn(**{which: lambda p: ir.flip(p.input(which, (6, 2, 16, 64), ir.BF16), 2)})
+    assert p.emit(0)[0] == "operator:paged_attn[plain]"
+    p = attn(**{which: lambda p: ir.flip(p.input(which, (6, 2, 16, 64), ir.BF16), 1)})
+    assert p.emit(0)[0] == "operator:paged_attn[mfma]"
+
+
 def _computed_k():
     p = Program()
     k = ir.map_(ir.MUL, p.input("k", (5, 2, 16)), ir.const(2.0))

@@ -48,7 +48,7 @@ def run_alone(body):
     return mark
 
 
-def attention(t, folder, run_in, starts=None, order=0, math=True, **kw):
+def attention(t, folder, run_in, starts=None, order=0, math=True, change=lambda text: text, **kw):
     """The batch's output [T, NH, HD] and the kernel's kind; fails where the kernel goes out of bounds."""
     kind, source = t.program(**kw).emit(0)
     c = host.constants(source)
@@ -60,7 +60,7 @@ def attention(t, folder, run_in, starts=None, order=0, math=True, **kw):
         q = q.transpose(1, 0, 2)
     ops, grid = host.attention_operands(c, encode(q, dq), encode(kc, dc), encode(vc, dc), t.tables, t.starts if starts is None else starts,
                                         t.past, t.q.size * ir.dtype_bytes(do, 1))
-    why = host.run(host.build(source, str(folder), math), str(run_in), grid, ops, order)
+    why = host.run(host.build(source, str(folder), math, change), str(run_in), grid, ops, order)
     assert why is None, why
     if len(ops) > 7:
         assert not any(ops[8]), "arrivals are left over for the next launch"
@@ -124,7 +124,7 @@ def test_mixed_batches_stay_in_bounds(seed, results, request):
     results[request.node.name].result()
 
 
-def test_what_the_host_run_notices(folder, tmp_path, monkeypatch):
+def test_what_the_host_run_notices(folder, tmp_path):
     """A buffer that ends early, a tile read before it has arrived, a part of LDS that is not there."""
     t = Batch(**ATTN["decode"])
     with pytest.raises(AssertionError, match="operand 1 at byte"):
@@ -132,15 +132,13 @@ def test_what_the_host_run_notices(folder, tmp_path, monkeypatch):
         t.kc = kc[:int(t.tables[0, 0])]     # the pool ends ahead of a block in use
         attention(t, folder, tmp_path)
     t.kc = kc
-    text = host.host_text
     for old, new, said in (("wh::turn_barrier(0)", "wh::turn_barrier(99)", None),
                            ("n * 512], 16, 0, 0)", "n * 512 + RING], 16, 0, 0)", "signal 4|outside its ring")):
-        def changed(source):
-            assert old in text(source)
-            return text(source).replace(old, new)
-        monkeypatch.setattr(host, "host_text", changed)
+        def change(text):
+            assert old in text
+            return text.replace(old, new)
         with pytest.raises(AssertionError, match=said):
-            t.check(*attention(t, folder, tmp_path))
+            t.check(*attention(t, folder, tmp_path, change=change))
 
 
 def _words(x):

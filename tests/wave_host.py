@@ -59,9 +59,9 @@ def host_text(source):
     return (f'#include "{HERE}/wave_host.hpp"\n{text}\n#define KERNEL {name}\n#define RING {ring}\n#include "{HERE}/wave_host_main.hpp"\n')
 
 
-def build(source, folder, math=True):
+def build(source, folder, math=True, change=lambda text: text):
     """The executable of a kernel's text, made once per text in `folder`."""
-    text = host_text(source)
+    text = change(host_text(source))
     headers = "".join(open(os.path.join(HERE, n)).read() for n in ("wave_host.hpp", "wave_host_main.hpp"))
     exe = os.path.join(folder, "k" + hashlib.sha256((text + headers + str(math)).encode()).hexdigest()[:20])
     if not os.path.exists(exe):

@@ -59,7 +59,9 @@ extern "C" __global__ void __launch_bounds__(256) sanic_paged_attn(Args a) {
     const float top = __builtin_fmaxf(m, sanic_wave_max(s));
     // nothing seen so far, or only scores of -inf (whose weights are 0): no reference to subtract
     const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
-    const float w = seen ? __expf(s - ref) : 0.0f, c = __expf(m - ref);
+    // (above 0, so that an infinite value among the earlier ones stays one: next to the weight of 1 that
+    // moved the reference, 2^-126 is nothing)
+    const float w = seen ? __expf(s - ref) : 0.0f, c = __builtin_fmaxf(__expf(m - ref), 0x1p-126f);
     m = top;
     sum = sum * c + sanic_wave_sum(w);
     for (int i = 0; i < DV; i++) o[i] *= c;
@@ -70,7 +72,7 @@ extern "C" __global__ void __launch_bounds__(256) sanic_paged_attn(Args a) {
       const unsigned pg = page_of[wave][x];
       if (pg >= NB) continue;   // a masked place's value may be anything, NaN among it
       const kv_t* v = a.v + (VB + pg * V0 + g * V1 + (base + x) % BS * V2);
-      const float wx = w_of[wave][x];
+      const float wx = __builtin_fmaxf(w_of[wave][x], 0x1p-126f);   // a weight that is 0 in 32 bits is none of a seen key
       for (int i = 0; i < DV; i++)
         if (lane + 64 * i < HD) o[i] = __builtin_fmaf(wx, sanic_get<DC>(v[(lane + 64 * i) * V3]), o[i]);
     }
@@ -186,7 +188,7 @@ __shared__ struct {
   __attribute__((aligned(1024))) unsigned short ring[RING];
   unsigned pages[PAGES];
   unsigned long long odd_keys;
-  int holes, last_arrival;
+  int holes, last_arrival, not_finite;
 } lds;
 
 // ── what this workgroup does ──────────────────────────────────────────────────────────────────────
@@ -295,7 +297,7 @@ __device__ __forceinline__ void find_many(const Args& a, const Plan& p, Req& q, 
 struct Stream {
   const Args& a;
   const unsigned* table;
-  int g, first_page, last_page, base;   // the pages seen by any row; the first page in LDS
+  int tid, g, first_page, last_page, base;   // the thread; the pages seen by any row; the first page in LDS
   const unsigned short *k, *v;
 
   // the block table from page p on into LDS (every thread, between two barriers)
@@ -312,7 +314,7 @@ struct Stream {
   }
   template <class R> __device__ __forceinline__ bool covers(int t0) const { return t0 / BS >= base && (t0 + R::TK - 1) / BS < base + PAGES; }
   template <class R> __device__ __forceinline__ void fetch(int t0, int buf) const {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int row = lane >> 2, c = (lane & 3) ^ (row >> 1 & 3);
     // 16 rows of one page: its address is the wave's, a lane's part of it the same in every tile
     unsigned page_of[R::LOADS];
@@ -371,7 +373,7 @@ __device__ __forceinline__ void need(Stream& st, int t0) {
 // is anyway): the compiler would otherwise wait for them, and so for every tile, inside the loop.
 template <class R, int RT>
 __device__ __forceinline__ void begin(Stream& st, int t_first, int t_last, s16x8 (&q)[RT][DSTEP]) {
-  if (threadIdx.x == 0) lds.holes = 0;
+  if (threadIdx.x == 0) lds.holes = 0, lds.not_finite = 0;
   __syncthreads();
   if (t_first < t_last) st.pages_from(t_first * R::TK / BS);
   #pragma unroll
@@ -426,6 +428,10 @@ __device__ __forceinline__ void tr_read8(unsigned even, s16x4 (&r)[8]) {
 }
 __device__ __forceinline__ bool odd_value(unsigned short x) { return HALF ? (x & 0x7C00) == 0x7C00 : (x & 0x7F80) == 0x7F80; }
 
+// What earlier sums are scaled by when the reference moves by -x: 2^x, but never 0, which would make NaN of
+// an infinite sum (next to the weight of 1 or more that moved the reference, 2^-126 is nothing).
+__device__ __forceinline__ float decay(float x) { return __builtin_fmaxf(__builtin_amdgcn_exp2f(x), 0x1p-126f); }
+
 // One column of scores into weights: s holds the products of the tile's keys row0 + 16·kt + r, of which
 // the row sees those in [lo, hi) that are no holes, and leaves as 2^(t − m). `factor` is what the row's earlier sums are scaled by.
 template <int N>
@@ -450,20 +456,32 @@ __device__ __forceinline__ void weigh(f32x4 (&s)[N], bool full, unsigned long lo
   if (!__all(top <= m + 8.0f && m > NEG_INF)) {
     top = quad_max(top);
     const float to = top > m + 8.0f ? top : m;
-    factor = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+    factor = to == m ? 1.0f : decay(m - to);
     m = to;
   }
   // nothing seen so far, or scores of −inf alone: their weights are 0, 2^(−inf − 0)
   const float ref = m == NEG_INF ? 0.0f : m;
-  #pragma unroll
-  for (int kt = 0; kt < N; kt++)
+  // (a branch for the whole tile, or a choice for each score, by what the compiler makes of them: heads of
+  // 128, 4096 rows 1187 us against 1238; heads of 64, a mixed batch 65.8 against 55.2)
+  if (HD > 64 && full) {
     #pragma unroll
-    for (int r = 0; r < 4; r++) s[kt][r] = __builtin_amdgcn_exp2f(full ? __builtin_fmaf(s[kt][r], C2, -ref) : s[kt][r] - ref);
+    for (int kt = 0; kt < N; kt++)
+      #pragma unroll
+      for (int r = 0; r < 4; r++) s[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], C2, -ref));
+  } else {
+    #pragma unroll
+    for (int kt = 0; kt < N; kt++)
+      #pragma unroll
+      for (int r = 0; r < 4; r++) s[kt][r] = __builtin_amdgcn_exp2f(full ? __builtin_fmaf(s[kt][r], C2, -ref) : s[kt][r] - ref);
+  }
 }
 
 // Values that nobody in the workgroup sees become 0 (0·NaN would reach every row of the product);
 // where one that is seen is not finite, its key's bit is returned, and it is 0 in the tile: add_odd
-// adds it to the rows that see it. Rows [row0, row0 + rows) × chunks [c0, c0 + chunks), of which any row
+// adds it to the rows that see it. Tiles that every row sees whole are not cleaned: there a value that
+// is not finite goes through the product, which may make NaN of an infinite one (by a weight that is 0
+// in 32 bits, by the negative rest of a weight's first term). Rows whose sums come out not finite are
+// computed again with every tile cleaned. Rows [row0, row0 + rows) × chunks [c0, c0 + chunks), of which any row
 // sees [lo, hi) (rows counted from the tile's first key).
 __device__ __forceinline__ unsigned long long clean(int tile, unsigned long long holes, int row0, int rows, int c0, int chunks, int lo, int hi, int part, int parts) {
   unsigned long long odd = 0;
@@ -484,18 +502,14 @@ __device__ __forceinline__ unsigned long long clean(int tile, unsigned long long
   }
   return odd;
 }
-template <int N, int D>
-__device__ __forceinline__ void add_odd(const Stream& st, unsigned long long odd, int t0, int rel, const f32x4 (&w)[N], f32x4 (&o)[D], int dt0, int lq) {
+// The values of the tile's keys `odd` that are not finite, to the rows that see those keys: a weight above
+// 0, however small, leaves such a value what it is.
+template <int D>
+__device__ __forceinline__ void add_odd(const Stream& st, unsigned long long odd, int t0, int lo, int hi, f32x4 (&o)[D], int dt0, int lq) {
   while (odd) {
     const int row = __builtin_ctzll(odd), key = t0 + row;
     odd &= odd - 1;
-    float x = 0.0f;
-    #pragma unroll
-    for (int kt = 0; kt < N; kt++)
-      #pragma unroll
-      for (int r = 0; r < 4; r++)
-        if (rel + kt * 16 + lq * 4 + r == row) x = w[kt][r];
-    x = sanic_rows_sum(x);
+    const bool seen = row >= lo && row < hi;
     const unsigned page = st.table[key / BS];
     const unsigned short* v = st.v + ((long long)page * V0 + key % BS * V2);
     #pragma unroll
@@ -505,12 +519,18 @@ __device__ __forceinline__ void add_odd(const Stream& st, unsigned long long odd
       struct __attribute__((packed, aligned(4))) run { unsigned short e[4]; };
       const run y = *(const run*)(v + col);
       #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const float z = x * sanic_get<DQ>(__builtin_bit_cast(sanic_elem<DQ>::T, y.e[r]));
-        o[d][r] += odd_value(y.e[r]) && x != 0.0f ? z : 0.0f;
-      }
+      for (int r = 0; r < 4; r++)
+        o[d][r] += seen && odd_value(y.e[r]) ? sanic_get<DQ>(__builtin_bit_cast(sanic_elem<DQ>::T, y.e[r])) : 0.0f;
     }
   }
+}
+template <int N> __device__ __forceinline__ bool not_finite(const f32x4 (&o)[N], const f32x4& sum) {
+  f32x4 x = sum * 0.0f;
+  #pragma unroll
+  for (int d = 0; d < N; d++)
+    #pragma unroll
+    for (int r = 0; r < 4; r++) x[r] = __builtin_fmaf(o[d][r], 0.0f, x[r]);
+  return (x[0] + x[1]) + (x[2] + x[3]) != 0.0f;     // NaN
 }
 
 // ── the parts of a row ────────────────────────────────────────────────────────────────────────────
@@ -560,7 +580,7 @@ __device__ __forceinline__ void meet(const Args& a, const Item& it, int g, int r
     float m = NEG_INF, l = 0.0f;
     auto add = [&](float m2, float l2, f32x4 v) {
       const float to = __builtin_fmaxf(m, m2), ref = to == NEG_INF ? 0.0f : to;   // (a split that saw nothing has weight 0)
-      const float f = __builtin_amdgcn_exp2f(m - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+      const float f = decay(m - ref), f2 = decay(m2 - ref);
       acc = acc * f + v * f2;
       l = l * f + l2 * f2;
       m = to;
@@ -605,9 +625,9 @@ __device__ __forceinline__ void few_values(unsigned at, s16x4 (&vt)[(DTH + 3) / 
 
 // ── few rows: the waves split the tile's keys ─────────────────────────────────────────────────────
 template <int RT>
-__device__ __forceinline__ void few_rows(const Args& a, const Item& it, int stride, int g, Stream& st, int t_first, int t_last, int lo_all, int hi_all, int full_lo, int full_hi) {
+__device__ __forceinline__ bool few_rows(const Args& a, const Item& it, int stride, int g, Stream& st, int t_first, int t_last, int lo_all, int hi_all, int full_lo, int full_hi, bool careful) {
   constexpr int TK = FEW_TK;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
+  const int tid = st.tid, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
   const int kg = wave % KG, dh = wave / KG, dt0 = dh * DTH;
   s16x8 qf[RT][DSTEP];
   int lo[RT], hi[RT];
@@ -636,7 +656,7 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int stri
     const int t0 = i * TK;
     turn<Few>(st, i, t_last, buf);
     const unsigned long long holes = lds.holes ? st.missing<TK>(t0) : 0;
-    const bool full = t0 >= full_lo && t0 + TK <= full_hi && !holes;
+    const bool full = !careful && t0 >= full_lo && t0 + TK <= full_hi && !holes;
     unsigned long long odd = 0;
     if (!full) {
       const int c0 = dt0 * 2, c1 = (dt0 + DTH) * 2 < CH ? (dt0 + DTH) * 2 : CH;
@@ -658,7 +678,7 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int stri
         for (int d = 0; d < DTH; d++) o[t][d] *= factor;
       }
       if (t == 0) few_values<0>(value_at(Few::at(buf, 1), l16, lq) + (kg * CG + (dt0 >> 1)) * 1024, vt);
-      if (odd) add_odd<1, DTH>(st, odd, t0, kg * 16, s, o[t], dt0, lq);
+      if (odd) add_odd<DTH>(st, odd, t0, lo[t] - t0, hi[t] - t0, o[t], dt0, lq);
       #pragma unroll
       for (int k = 0; k < FEW_TERMS; k++) {
         const s16x4 p = __builtin_bit_cast(s16x4, pack(s[0]));
@@ -669,8 +689,13 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int stri
     }
     buf = buf == Few::ST - 1 ? 0 : buf + 1;
   }
+  bool bad = false;
+  #pragma unroll
+  for (int t = 0; t < RT; t++) bad |= not_finite(o[t], sum[t]);
+  if (bad && !careful) lds.not_finite = 1;
   // the key groups meet: maxima and sums, then the outputs, group after group
   __syncthreads();
+  if (!careful && __builtin_amdgcn_readfirstlane(lds.not_finite)) return true;
   float* stat = (float*)lds.pages;                       // [2][KG][16·RT], by the waves of the first dims
   float* acc = (float*)lds.ring;                         // [KG][16·RT][HD]
   if (dh == 0 && lq == 0) {
@@ -683,7 +708,7 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int stri
     const int row = t * 16 + l16;
     float mx = NEG_INF;
     for (int k = 0; k < KG; k++) mx = __builtin_fmaxf(mx, stat[k * 32 + row]);
-    const float f = mx == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m[t] - mx);
+    const float f = mx == NEG_INF ? 0.0f : decay(m[t] - mx);
     #pragma unroll
     for (int d = 0; d < DTH; d++)
       if (dt0 + d < DT) *(f32x4*)&acc[(kg * 16 * RT + row) * HD + (dt0 + d) * 16 + lq * 4] = o[t][d] * f;
@@ -708,6 +733,7 @@ __device__ __forceinline__ void few_rows(const Args& a, const Item& it, int stri
     }
   }
   if (it.splits > 1) meet(a, it, g, 0, it.rows, 2 * stride, stride);
+  return false;
 }
 
 // Oᵀ += Vᵀ·P over the tile, eight reads (all keys of two or four tiles of dims) at a time
@@ -736,9 +762,9 @@ __device__ __forceinline__ void many_values(unsigned at, const s16x8 (&p)[2][MAN
 }
 
 // ── many rows: 32 a wave ──────────────────────────────────────────────────────────────────────────
-__device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, Stream& st, int t_first, int t_last, int lo_all, int hi_all, int full_lo, int full_hi) {
+__device__ __forceinline__ bool many_rows(const Args& a, const Item& it, int g, Stream& st, int t_first, int t_last, int lo_all, int hi_all, int full_lo, int full_hi, bool careful) {
   constexpr int TK = MANY_TK, NK = TK / 16;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
+  const int tid = st.tid, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
   const int row0 = it.tile * PR + wave * 32;
   s16x8 qf[2][DSTEP];
   int lo[2], hi[2];
@@ -773,7 +799,7 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
     turn<Many>(st, i, t_last, buf);
     const unsigned long long holes = lds.holes ? st.missing<TK>(t0) : 0;
     unsigned long long odd = 0;
-    if (!(t0 >= full_lo && t0 + TK <= full_hi) || holes) {
+    if (!(t0 >= full_lo && t0 + TK <= full_hi) || holes || careful) {
       // the tile is every wave's: cleaned by all, then used
       if (tid == 0) lds.odd_keys = 0;
       __syncthreads();
@@ -783,7 +809,7 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
       odd = lds.odd_keys;
     }
     if (!idle && t0 < wave_hi && t0 + TK > wave_lo) {
-      const bool full = t0 >= all_lo && t0 + TK <= all_hi && !holes;
+      const bool full = !careful && t0 >= all_lo && t0 + TK <= all_hi && !holes;
       f32x4 s[2][NK];
       #pragma unroll
       for (int kt = 0; kt < NK; kt++) {
@@ -805,7 +831,7 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
           #pragma unroll
           for (int d = 0; d < DT; d++) o[t][d] *= factor;
         }
-        if (odd) add_odd<NK, DT>(st, odd, t0, 0, s[t], o[t], 0, lq);
+        if (odd) add_odd<DT>(st, odd, t0, lo[t] - t0, hi[t] - t0, o[t], 0, lq);
         #pragma unroll
         for (int ks = 0; ks < NK / 2; ks++)
           #pragma unroll
@@ -819,6 +845,9 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
     }
     buf = buf == Many::ST - 1 ? 0 : buf + 1;
   }
+  if (!careful && (not_finite(o[0], sum[0]) || not_finite(o[1], sum[1]))) lds.not_finite = 1;
+  __syncthreads();
+  if (!careful && __builtin_amdgcn_readfirstlane(lds.not_finite)) return true;
   const int tile_rows = it.rows - it.tile * PR < PR ? it.rows - it.tile * PR : PR;
   #pragma unroll
   for (int t = 0; t < 2; t++) {
@@ -840,24 +869,30 @@ __device__ __forceinline__ void many_rows(const Args& a, const Item& it, int g, 
     }
   }
   if (it.splits > 1) meet(a, it, g, it.tile * PR, tile_rows, PR, 0);
+  return false;
 }
 
-// Rows [r0, r1) of an item: what any and what all of them see, and the part of the key tiles.
+// Rows [r0, r1) of an item: what any and what all of them see, and the part of the key tiles. True where
+// a sum came out not finite: nothing has been stored then, and the rows are taken again, with `careful`
+// (from here, not inside: what a second pass keeps in registers would cost the first one its own).
 template <bool MANY>
-__device__ __forceinline__ void rows_of(const Args& a, const Item& it, int g, int r0, int r1, int t0, int t1, int stride) {
+__device__ __forceinline__ bool rows_of(const Args& a, const Item& it, int g, int r0, int r1, int t0, int t1, int stride, bool careful) {
   constexpr int TK = MANY ? MANY_TK : FEW_TK;
   const long long p0 = it.past + r0 / REP, p1 = it.past + (r1 - 1) / REP;
   const int hi_all = clamp_pos(p1 + 1), full_hi = clamp_pos(p0 + 1);
   const int lo_all = W ? clamp_pos(p0 + 1 - W) : 0, full_lo = W ? clamp_pos(p1 + 1 - W) : 0;
   const int k0 = lo_all / TK, k1 = lo_all < hi_all ? (hi_all + TK - 1) / TK : k0;
-  Stream st{a, a.tables + (long long)it.b * M, g, lo_all / BS, (hi_all - 1) / BS, 0, a.k + (KB + g * K1), a.v + (VB + g * V1)};
+  // (an opaque copy, so that nothing a lane computes from it is kept in registers around a second pass)
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  Stream st{a, a.tables + (long long)it.b * M, tid, g, lo_all / BS, (hi_all - 1) / BS, 0, a.k + (KB + g * K1), a.v + (VB + g * V1)};
   if constexpr (MANY) {
     const int t_first = k0 + (int)((long long)(k1 - k0) * it.split / it.splits), t_last = k0 + (int)((long long)(k1 - k0) * (it.split + 1) / it.splits);
-    many_rows(a, it, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
+    return many_rows(a, it, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi, careful);
   } else {
     const int t_first = k0 + t0 < k1 ? k0 + t0 : k1, t_last = k0 + t1 < k1 ? k0 + t1 : k1;
-    if (it.rows <= 16) few_rows<1>(a, it, stride, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
-    else few_rows<2>(a, it, stride, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi);
+    if (it.rows <= 16) return few_rows<1>(a, it, stride, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi, careful);
+    return few_rows<2>(a, it, stride, g, st, t_first, t_last, lo_all, hi_all, full_lo, full_hi, careful);
   }
 }
 
@@ -871,7 +906,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) sanic_paged_attn(Args a) 
   if (PITEMS && w < p.items) {
     find_many(a, p, q, w, it);
     const int r0 = it.tile * PR, r1 = r0 + PR < it.rows ? r0 + PR : it.rows;
-    rows_of<true>(a, it, g, r0, r1, 0, 0, 0);
+    for (bool careful = false; rows_of<true>(a, it, g, r0, r1, 0, 0, 0, careful); careful = true) __syncthreads();
     return;
   }
   // the requests in the w-th run of key tiles
@@ -890,7 +925,8 @@ extern "C" __global__ void __launch_bounds__(256, OCC) sanic_paged_attn(Args a) 
       it.slot = w0 * 2 * p.stride;             // a request's first part is its workgroup's second partial
       it.count = it.b;
       it.start = pick(q.start, l), it.past = pick(q.past, l);
-      rows_of<false>(a, it, g, 0, it.rows, (r0 > from ? r0 : from) - from, (r1 < to ? r1 : to) - from, p.stride);
+      const int t0 = (r0 > from ? r0 : from) - from, t1 = (r1 < to ? r1 : to) - from;
+      for (bool careful = false; rows_of<false>(a, it, g, 0, it.rows, t0, t1, p.stride, careful); careful = true) __syncthreads();
       __syncthreads();
     }
     before = pick(inc, 63);

@@ -1,0 +1,41 @@
+"""Batches whose values are not finite, with what the definition gives for them."""
+import numpy as np
+
+from sanic_amd import ir
+from test_gpu_operators import Batch, stored
+
+
+class OddValue:
+    """One value of a key that stands in a tile every row sees whole, and its effect: a value that is
+    not finite reaches that dim of every row that sees its key, whatever the key's weight, and nothing
+    else."""
+
+    def __init__(self, value, at, far=False, HD=64, past=200, new=1, dim=5, dq=ir.BF16, do=None, rep=4, NKV=2):
+        kw = dict(past=[past, 40], new=[new, new], NKV=NKV, rep=rep, HD=HD, BS=16, dq=dq, do=do)
+        self.batch, self.clean = Batch(**kw), Batch(**kw)
+        where = (int(self.batch.tables[0, at // 16]), slice(None), at % 16)
+        if far:       # a score so far below the others that the weight is 0 in 32 bits
+            for t in (self.batch, self.clean):
+                t.q[:, :, 0] = 8.0
+                t.kc[where + (0,)] = stored(-400.0, dq)
+        self.clean.vc[where + (dim,)] = 0.0
+        self.batch.vc[where + (dim,)] = value
+        self.value, self.dim, self.at = value, dim, at
+
+    def check(self, got, kind):
+        t = self.batch
+        rows = slice(0, t.new[0])
+        seen = got[rows][..., self.dim]
+        assert np.isnan(seen).all() if np.isnan(self.value) else (seen == self.value).all(), seen.ravel()[:8]
+        got = got.copy()
+        got[rows][..., self.dim] = self.clean.want()[0][rows][..., self.dim]
+        self.clean.check(got, kind)
+
+
+ODD_VALUES = {
+    f"{n}_{np.format_float_positional(v, trim='-')}{'_far' if far else ''}": dict(kw, value=v, far=far)
+    for n, kw in {
+        "token": dict(at=70), "token_128": dict(at=70, HD=128), "token_f16": dict(at=70, dq=ir.F16), "drafts": dict(at=33, new=5), "drafts_80": dict(at=33, new=5, HD=80),
+        "token_f32_out": dict(at=70, do=ir.F32), "chunk": dict(at=70, new=60), "chunk_128": dict(at=70, new=40, HD=128), "chunk_f32_out": dict(at=70, new=60, do=ir.F32),
+        "chunk_f16": dict(at=70, new=60, dq=ir.F16), "head_24": dict(at=70, HD=24), "first_key": dict(at=0, new=40), "split": dict(at=600, past=4000, rep=2, NKV=1),
+    }.items() for v in (np.inf, -np.inf, np.nan) for far in (False, True)}

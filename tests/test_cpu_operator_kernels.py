@@ -10,6 +10,7 @@ import pytest
 
 import paged_ref as ref
 import wave_host as host
+from paged_cases import ODD_VALUES, OddValue
 from sanic_amd import ir
 from sanic_amd.backend import decode, encode
 from sanic_amd.program import NONE
@@ -139,6 +140,17 @@ def test_what_the_host_run_notices(folder, tmp_path):
             return text.replace(old, new)
         with pytest.raises(AssertionError, match=said):
             t.check(*attention(t, folder, tmp_path, change=change))
+
+
+def _odd_value(case, folder, run_in):
+    odd = OddValue(**ODD_VALUES[case])
+    odd.check(*attention(odd.batch, folder, run_in))
+
+
+@run_alone(_odd_value)
+@pytest.mark.parametrize("case", ODD_VALUES)
+def test_a_value_not_finite_in_the_past(case, results, request):
+    results[request.node.name].result()
 
 
 def _words(x):

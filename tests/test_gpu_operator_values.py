@@ -1,0 +1,22 @@
+"""The operators where values, indices or lengths are at the edge of what they may be, on the GPU: the
+cases of tests/test_cpu_operator_kernels.py again."""
+import pytest
+
+from paged_cases import ODD_VALUES, OddValue
+from test_gpu_operators import bind, read
+
+pytestmark = pytest.mark.gpu
+
+
+def attention(dev, t):
+    p = t.program()
+    bufs = bind(dev, p, t.values())
+    exe = dev.prepare(p)
+    exe.execute_static(bufs)
+    return read(p, bufs, "o"), exe.stage_kernel(0)
+
+
+@pytest.mark.parametrize("case", ODD_VALUES)
+def test_a_value_not_finite_in_the_past(dev, case):
+    odd = OddValue(**ODD_VALUES[case])
+    odd.check(*attention(dev, odd.batch))

@@ -331,7 +331,7 @@ struct Stream {
       const int cg = n % CG * 4;
       int chunk = c;
       if (R::TK / 16 * CG % 4 && group >= R::TK / 16) group = R::TK / 16 - 1;
-      if (CH % 4 && cg + c >= CH) chunk = CH - 1 - cg;    // (the query is 0 there)
+      if (CH % 4 && cg + c >= CH) chunk = CH - 1 - cg;    // (read as 0 by key_run)
       const unsigned key = (unsigned)t0 + group * 16;
       // a page that is none is read as block 0 and masked
       const char *kp, *vp;
@@ -403,7 +403,11 @@ __device__ __forceinline__ void turn(Stream& st, int t, int t_last, int buf) {
 }
 
 __device__ __forceinline__ s16x8 key_run(int tile, int group, int step, int l16, int lq) {
-  return *(const s16x8*)&lds.ring[tile + (group * CG + step) * 512 + in_block(l16, lq)];
+  s16x8 x = *(const s16x8*)&lds.ring[tile + (group * CG + step) * 512 + in_block(l16, lq)];
+  // behind a head's end stand copies of other dims, which need not be finite, and the query's 0 would not
+  // take those out of the product
+  if (HD % 32 && step == DSTEP - 1 && step * 4 + lq >= CH) x = (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
+  return x;
 }
 // Transposed reads of 16 keys × 16 value dims: a lane gets 4 keys of one dim. A lane's place in a block
 // for an even tile of dims; for an odd one it is 32 bytes further or back (two chunks, swapped alike).

@@ -39,3 +39,28 @@ ODD_VALUES = {
         "token_f32_out": dict(at=70, do=ir.F32), "chunk": dict(at=70, new=60), "chunk_128": dict(at=70, new=40, HD=128), "chunk_f32_out": dict(at=70, new=60, do=ir.F32),
         "chunk_f16": dict(at=70, new=60, dq=ir.F16), "head_24": dict(at=70, HD=24), "first_key": dict(at=0, new=40), "split": dict(at=600, past=4000, rep=2, NKV=1),
     }.items() for v in (np.inf, -np.inf, np.nan) for far in (False, True)}
+
+
+class OddKey:
+    """One key with an element of −inf against queries that are positive there: a score of −inf, so a
+    weight of 0, and every row is as if the key were not there. The others see their own keys."""
+
+    def __init__(self, HD, dim, new=1, at=70, dq=ir.BF16, value=-np.inf):
+        kw = dict(past=[200, 40], new=[new, new], NKV=2, rep=4, HD=HD, BS=16, dq=dq)
+        self.batch, self.clean = Batch(**kw), Batch(**kw)
+        where = (int(self.batch.tables[0, at // 16]), slice(None), at % 16)
+        for t in (self.batch, self.clean):
+            t.q[:, :, dim] = np.abs(t.q[:, :, dim]) + 0.5
+            t.q[:] = stored(t.q, dq)
+        self.batch.kc[where + (dim,)] = value
+        # so far below the others that its weight is 0 in 64 bits too
+        self.clean.kc[where + (dim,)] = stored(-60000.0, dq)
+
+    def check(self, got, kind):
+        assert np.isfinite(got).all(), np.argwhere(~np.isfinite(got))[:4]
+        self.clean.check(got, kind)
+
+
+ODD_KEYS = {f"head_{HD}_dim_{dim}_rows_{new}_{'f16' if dq == ir.F16 else 'bf16'}": dict(HD=HD, dim=dim, new=new, dq=dq)
+            for HD, dim in ((16, 15), (48, 40), (80, 72), (112, 111), (144, 137), (208, 207), (64, 63), (24, 23)) for new in (1, 5, 50)
+            for dq in ((ir.BF16, ir.F16) if HD == 80 else (ir.BF16,))}

@@ -10,7 +10,7 @@ import pytest
 
 import paged_ref as ref
 import wave_host as host
-from paged_cases import ODD_VALUES, OddValue
+from paged_cases import ODD_KEYS, ODD_VALUES, OddKey, OddValue
 from sanic_amd import ir
 from sanic_amd.backend import decode, encode
 from sanic_amd.program import NONE
@@ -150,6 +150,17 @@ def _odd_value(case, folder, run_in):
 @run_alone(_odd_value)
 @pytest.mark.parametrize("case", ODD_VALUES)
 def test_a_value_not_finite_in_the_past(case, results, request):
+    results[request.node.name].result()
+
+
+def _odd_key(case, folder, run_in):
+    odd = OddKey(**ODD_KEYS[case])
+    odd.check(*attention(odd.batch, folder, run_in))
+
+
+@run_alone(_odd_key)
+@pytest.mark.parametrize("case", ODD_KEYS)
+def test_a_key_of_minus_infinity_has_no_weight(case, results, request):
     results[request.node.name].result()
 
 

@@ -2,7 +2,7 @@
 cases of tests/test_cpu_operator_kernels.py again."""
 import pytest
 
-from paged_cases import ODD_VALUES, OddValue
+from paged_cases import ODD_KEYS, ODD_VALUES, OddKey, OddValue
 from test_gpu_operators import bind, read
 
 pytestmark = pytest.mark.gpu
@@ -19,4 +19,10 @@ def attention(dev, t):
 @pytest.mark.parametrize("case", ODD_VALUES)
 def test_a_value_not_finite_in_the_past(dev, case):
     odd = OddValue(**ODD_VALUES[case])
+    odd.check(*attention(dev, odd.batch))
+
+
+@pytest.mark.parametrize("case", ODD_KEYS)
+def test_a_key_of_minus_infinity_has_no_weight(dev, case):
+    odd = OddKey(**ODD_KEYS[case])
     odd.check(*attention(dev, odd.batch))

@@ -722,7 +722,8 @@ __device__ __forceinline__ bool few_rows(const Args& a, const Item& it, int stri
     const int row = u / (HD / 4), d = u % (HD / 4) * 4;
     float mx = NEG_INF, l = 0.0f;
     for (int k = 0; k < KG; k++) mx = __builtin_fmaxf(mx, stat[k * 32 + row]);
-    for (int k = 0; k < KG; k++) l += mx == NEG_INF ? 0.0f : stat[128 + k * 32 + row] * __builtin_amdgcn_exp2f(stat[k * 32 + row] - mx);
+    // (scores that are all NaN leave no maximum, and sums of NaN)
+    for (int k = 0; k < KG; k++) l += stat[128 + k * 32 + row] * (mx == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(stat[k * 32 + row] - mx));
     f32x4 v = *(const f32x4*)&acc[row * HD + d];
     for (int k = 1; k < KG; k++) v += *(const f32x4*)&acc[(k * 16 * RT + row) * HD + d];
     if (it.splits == 1) {

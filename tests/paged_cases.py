@@ -64,3 +64,27 @@ class OddKey:
 ODD_KEYS = {f"head_{HD}_dim_{dim}_rows_{new}_{'f16' if dq == ir.F16 else 'bf16'}": dict(HD=HD, dim=dim, new=new, dq=dq)
             for HD, dim in ((16, 15), (48, 40), (80, 72), (112, 111), (144, 137), (208, 207), (64, 63), (24, 23)) for new in (1, 5, 50)
             for dq in ((ir.BF16, ir.F16) if HD == 80 else (ir.BF16,))}
+
+
+class OddQuery:
+    """A NaN in a query row makes the row NaN, and no other."""
+
+    def __init__(self, past, new, row, HD=64, NKV=2, rep=4, dq=ir.BF16, do=None):
+        self.batch = Batch(past=past, new=new, NKV=NKV, rep=rep, HD=HD, BS=16, dq=dq, do=do)
+        self.clean = Batch(past=past, new=new, NKV=NKV, rep=rep, HD=HD, BS=16, dq=dq, do=do)
+        self.row, self.head = row, NKV * rep - 1
+        self.batch.q[row, self.head, 3] = np.nan
+
+    def check(self, got, kind):
+        assert np.isnan(got[self.row, self.head]).all(), got[self.row, self.head][:8]
+        got = got.copy()
+        got[self.row, self.head] = self.clean.want()[0][self.row, self.head]
+        self.clean.check(got, kind)
+
+
+ODD_QUERIES = {
+    "first_token": dict(past=[0], new=[1], row=0), "token": dict(past=[70, 9], new=[1, 1], row=0), "token_split": dict(past=[4000, 9], new=[1, 1], row=0, NKV=1, rep=2),
+    "draft": dict(past=[70, 9], new=[5, 5], row=7), "draft_128": dict(past=[700, 9], new=[5, 5], row=3, HD=128), "draft_f32_out": dict(past=[70, 9], new=[5, 5], row=2, do=ir.F32),
+    "chunk": dict(past=[70, 9], new=[50, 5], row=13), "chunk_split": dict(past=[3000], new=[40], row=39, NKV=1), "head_80": dict(past=[70, 9], new=[5, 50], row=20, HD=80),
+    "head_24": dict(past=[70, 9], new=[5, 5], row=2, HD=24), "f16": dict(past=[70, 9], new=[5, 1], row=5, dq=ir.F16),
+}

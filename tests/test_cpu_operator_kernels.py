@@ -10,7 +10,7 @@ import pytest
 
 import paged_ref as ref
 import wave_host as host
-from paged_cases import ODD_KEYS, ODD_VALUES, OddKey, OddValue
+from paged_cases import ODD_KEYS, ODD_QUERIES, ODD_VALUES, OddKey, OddQuery, OddValue
 from sanic_amd import ir
 from sanic_amd.backend import decode, encode
 from sanic_amd.program import NONE
@@ -161,6 +161,17 @@ def _odd_key(case, folder, run_in):
 @run_alone(_odd_key)
 @pytest.mark.parametrize("case", ODD_KEYS)
 def test_a_key_of_minus_infinity_has_no_weight(case, results, request):
+    results[request.node.name].result()
+
+
+def _odd_query(case, folder, run_in):
+    odd = OddQuery(**ODD_QUERIES[case])
+    odd.check(*attention(odd.batch, folder, run_in))
+
+
+@run_alone(_odd_query)
+@pytest.mark.parametrize("case", ODD_QUERIES)
+def test_a_nan_in_a_query_is_in_its_row(case, results, request):
     results[request.node.name].result()
 
 

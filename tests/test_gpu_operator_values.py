@@ -2,7 +2,7 @@
 cases of tests/test_cpu_operator_kernels.py again."""
 import pytest
 
-from paged_cases import ODD_KEYS, ODD_VALUES, OddKey, OddValue
+from paged_cases import ODD_KEYS, ODD_QUERIES, ODD_VALUES, OddKey, OddQuery, OddValue
 from test_gpu_operators import bind, read
 
 pytestmark = pytest.mark.gpu
@@ -25,4 +25,10 @@ def test_a_value_not_finite_in_the_past(dev, case):
 @pytest.mark.parametrize("case", ODD_KEYS)
 def test_a_key_of_minus_infinity_has_no_weight(dev, case):
     odd = OddKey(**ODD_KEYS[case])
+    odd.check(*attention(dev, odd.batch))
+
+
+@pytest.mark.parametrize("case", ODD_QUERIES)
+def test_a_nan_in_a_query_is_in_its_row(dev, case):
+    odd = OddQuery(**ODD_QUERIES[case])
     odd.check(*attention(dev, odd.batch))

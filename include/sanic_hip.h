@@ -202,8 +202,8 @@ enum { SANIC_STAGE_FUSED = 0, SANIC_STAGE_POINTWISE = 1, SANIC_STAGE_OPERATOR = 
  *               tables[b], held[B] blocks are taken from `free`; a request with rows takes as many
  *               more, in the order of the requests, as its past + new positions need, as the table's
  *               M entries and the list's F blocks allow. Only the new entries of `tables` are
- *               written. A block id times BS fits 32 bits. slots[r] = block · BS + position mod BS, or SANIC_NONE without a block.
- *               B at most 8192.
+ *               written. slots[r] = block · BS + position mod BS, or SANIC_NONE where the position has
+ *               no block, its block is SANIC_NONE, or the slot would pass 32 bits. B at most 8192.
  * CACHE_WRITE   leaves k [T, NKV, HD], v [T, NKV, HD], slots [T], starts [B + 1], the key cache and
  *               the value cache (STATE, in place); output the key cache. Row r goes to slot slots[r]
  *               in the cache's type; slots of one step differ from each other.

@@ -45,6 +45,13 @@ __device__ __forceinline__ int last_at_most(const unsigned* a, int n, unsigned x
   return lo;
 }
 
+// a position's slot; none where its block is, or where the slot would not fit 32 bits (it would come out
+// as another, valid one)
+__device__ __forceinline__ unsigned slot_in(unsigned block, unsigned long long pos) {
+  const unsigned long long slot = (unsigned long long)block * BS + pos % BS;
+  return block != 0xFFFFFFFFu && slot < 0xFFFFFFFFu ? (unsigned)slot : 0xFFFFFFFFu;
+}
+
 __shared__ unsigned start_of[B + 1], block_of[B + 1];
 
 extern "C" __global__ void __launch_bounds__(256) sanic_block_tables(Args a) {
@@ -97,9 +104,9 @@ extern "C" __global__ void __launch_bounds__(256) sanic_block_tables(Args a) {
     unsigned slot = 0xFFFFFFFFu;
     // entries beyond those held are written by this launch: they are read from the list
     if (page < h) {
-      if (page < M) slot = a.tables[(long long)b * M + page] * (unsigned)BS + (unsigned)(pos % BS);
+      if (page < M) slot = slot_in(a.tables[(long long)b * M + page], pos);
     } else if (page - h < block_of[b + 1] - block_of[b]) {
-      slot = a.free[taken + block_of[b] + (page - h)] * (unsigned)BS + (unsigned)(pos % BS);
+      slot = slot_in(a.free[taken + block_of[b] + (page - h)], pos);
     }
     a.slots[r] = slot;
     a.positions[r] = (unsigned)pos;

@@ -151,7 +151,8 @@ class Program:
 
         Declares `<name>.starts` [B + 1] (request b has the rows from starts[b] to starts[b + 1]; cut
         at `rows`), `<name>.slots` and `<name>.positions` [rows] (slot = block·block size + offset,
-        NONE where no block is left; rows behind the last request are left as they were) and
+        NONE where no block is left, where the block is NONE and where the slot would pass 32 bits;
+        rows behind the last request are left as they were) and
         `<name>.held` [B + 1], `held` for the next step. Calling it again with the same inputs
         writes the same results. A request whose tokens were taken back (rejected drafts) keeps its
         blocks: `past` may fall, `held` stays."""

@@ -2,7 +2,8 @@
 import numpy as np
 
 from sanic_amd import ir
-from test_gpu_operators import Batch, stored
+from sanic_amd.program import NONE
+from test_gpu_operators import Batch, stored, tables_program
 
 
 class OddValue:
@@ -87,4 +88,46 @@ ODD_QUERIES = {
     "draft": dict(past=[70, 9], new=[5, 5], row=7), "draft_128": dict(past=[700, 9], new=[5, 5], row=3, HD=128), "draft_f32_out": dict(past=[70, 9], new=[5, 5], row=2, do=ir.F32),
     "chunk": dict(past=[70, 9], new=[50, 5], row=13), "chunk_split": dict(past=[3000], new=[40], row=39, NKV=1), "head_80": dict(past=[70, 9], new=[5, 50], row=20, HD=80),
     "head_24": dict(past=[70, 9], new=[5, 5], row=2, HD=24), "f16": dict(past=[70, 9], new=[5, 1], row=5, dq=ir.F16),
+}
+
+
+class LostBlocks:
+    """Block tables in whose lines, or whose free list, a block is none or lies past 32 bits of slots: its
+    positions have no slot."""
+
+    def __init__(self, table, free, past, new, block, M=4):
+        self.past, self.new, self.block, self.M, self.free = past, new, block, M, free
+        held = [-(-p // block) for p in past]
+        self.tables = np.full((len(past), M), NONE, np.int64)
+        for b, h in enumerate(held):
+            self.tables[b, :h] = table[b][:h]
+        self.held, self.T = held + [0], sum(new)
+
+    def program(self):
+        return tables_program(len(self.past), len(self.free), self.M, self.T, self.block)
+
+    def values(self):
+        return {"past": self.past, "new": self.new, "held": self.held, "free": self.free, "tables": self.tables}
+
+    def slots(self):
+        out, taken = [], 0
+        for b, (p, n) in enumerate(zip(self.past, self.new)):
+            line = list(self.tables[b][:self.held[b]])
+            while len(line) * self.block < p + n:
+                line.append(self.free[taken])
+                taken += 1
+            for pos in range(p, p + n):
+                at = int(line[pos // self.block]) * self.block + pos % self.block
+                out.append(NONE if line[pos // self.block] == NONE or at >= NONE else at)
+        return out
+
+
+LOST_BLOCKS = {
+    "none_held": dict(table=[[NONE], [7]], free=[3, 4], past=[5, 6], new=[2, 3], block=16),
+    "none_in_the_list": dict(table=[[9], [7]], free=[NONE, 4], past=[15, 16], new=[3, 2], block=16),
+    "past_32_bits": dict(table=[[1 << 28], [(1 << 28) - 1]], free=[(1 << 28) + 1, (1 << 32) - 2], past=[5, 8], new=[2, 3], block=16),
+    "past_32_bits_in_the_list": dict(table=[[1], [2]], free=[(1 << 28) + 1, (1 << 30) + 5], past=[15, 16], new=[9, 3], block=16),
+    "the_last_slots": dict(table=[[(1 << 28) - 1], [0xFFFFFFFF // 24]], free=[5], past=[13, 10], new=[3, 9], block=16),
+    "blocks_of_one": dict(table=[[NONE, NONE - 1], [5, 6]], free=[NONE - 1, NONE, 2], past=[2, 2], new=[1, 2], block=1),
+    "odd_block": dict(table=[[0xFFFFFFFF // 24], [0xFFFFFFFF // 24 + 1]], free=[5], past=[10, 3], new=[9, 9], block=24),
 }

@@ -10,7 +10,7 @@ import pytest
 
 import paged_ref as ref
 import wave_host as host
-from paged_cases import ODD_KEYS, ODD_QUERIES, ODD_VALUES, OddKey, OddQuery, OddValue
+from paged_cases import LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, LostBlocks, OddKey, OddQuery, OddValue
 from sanic_amd import ir
 from sanic_amd.backend import decode, encode
 from sanic_amd.program import NONE
@@ -203,6 +203,16 @@ def test_block_tables_on_the_cpu(B, seed, folder, tmp_path):
     n = starts[-1]
     assert _numbers(ops[8]).tolist() == starts and _numbers(ops[5])[:n].tolist() == slots and _numbers(ops[6])[:n].tolist() == positions
     assert _numbers(ops[7]).tolist() == [int(x) for x in after] and (_numbers(ops[4]).reshape(B, M) == want).all()
+
+
+@pytest.mark.parametrize("case", LOST_BLOCKS)
+def test_lost_blocks_have_no_slots(case, folder, tmp_path):
+    t = LostBlocks(**LOST_BLOCKS[case])
+    v, B = t.values(), len(t.past)
+    ops = [bytes(_words(v[n])) for n in ("past", "new", "held", "free")] + [_words(t.tables)] + [bytearray(4 * n) for n in (t.T, t.T, B + 1, B + 1)]
+    why = host.run(host.build(t.program().emit(0)[1], str(folder)), str(tmp_path), 1, ops)
+    assert why is None, why
+    assert _numbers(ops[5]).tolist() == t.slots()
 
 
 @pytest.mark.parametrize("HD,order,fused", [(16, "heads", False), (7, "tokens", False), (24, "tokens", True)])

@@ -2,8 +2,8 @@
 cases of tests/test_cpu_operator_kernels.py again."""
 import pytest
 
-from paged_cases import ODD_KEYS, ODD_QUERIES, ODD_VALUES, OddKey, OddQuery, OddValue
-from test_gpu_operators import bind, read
+from paged_cases import LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, LostBlocks, OddKey, OddQuery, OddValue
+from test_gpu_operators import bind, read, words
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,12 @@ def test_a_key_of_minus_infinity_has_no_weight(dev, case):
 def test_a_nan_in_a_query_is_in_its_row(dev, case):
     odd = OddQuery(**ODD_QUERIES[case])
     odd.check(*attention(dev, odd.batch))
+
+
+@pytest.mark.parametrize("case", LOST_BLOCKS)
+def test_lost_blocks_have_no_slots(dev, case):
+    t = LostBlocks(**LOST_BLOCKS[case])
+    p = t.program()
+    bufs = bind(dev, p, t.values())
+    dev.prepare(p).execute_static(bufs)
+    assert words(p, bufs, "plan.slots").tolist() == t.slots()

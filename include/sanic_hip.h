@@ -194,7 +194,8 @@ enum { SANIC_STAGE_FUSED = 0, SANIC_STAGE_POINTWISE = 1, SANIC_STAGE_OPERATOR = 
  * of NB blocks of BS tokens, [NB, NKV, BS, HD] for keys and for values; block tables[b][i] holds
  * request b's positions i·BS to i·BS + BS - 1. Counts, lengths, blocks and slots are U32 buffers;
  * SANIC_NONE stands for no block, slot or token, and every index is checked on the device: a block
- * or slot past the pool is none, a start past T is T.
+ * or slot past the pool is none, a start past T is T. Starts do not fall: where they do, PAGED_ATTN
+ * writes nothing, and VERIFY_DRAFTS takes each request as its own two starts say.
  *
  * BLOCK_TABLES  leaves past [B], new [B], held [B + 1], free [F], tables [B, M] (STATE, in place),
  *               slots [T], positions [T], held_next [B + 1]; output starts [B + 1]; stream = BS.

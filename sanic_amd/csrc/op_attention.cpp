@@ -31,6 +31,9 @@ extern "C" __global__ void __launch_bounds__(256) sanic_paged_attn(Args a) {
   const long long r = item / NH;
   const int h = (int)(item % NH), g = h / REP;
   if (r >= T || r >= a.starts[B]) return;
+  bool falls = false;
+  for (int i = lane; i < B; i += 64) falls |= a.starts[i + 1] < T && a.starts[i + 1] < a.starts[i];
+  if (__any(falls)) return;
   int b = 0, hi_b = B;   // the last request that starts at or before r
   while (hi_b - b > 1) {
     const int mid = (b + hi_b) >> 1;
@@ -199,11 +202,13 @@ struct Item {
 struct Req {
   long long start, past;
   int rows, tiles, kt;   // packed rows; workgroups of PR of them (0: few rows, D below); key tiles
+  bool falls;            // the request ends before it starts
 };
 __device__ __forceinline__ Req request(const Args& a, int b) {
-  Req q{0, 0, 0, 0, 0};
+  Req q{0, 0, 0, 0, 0, false};
   if (b >= B) return q;
   const long long s = a.starts[b] < T ? a.starts[b] : T, e = a.starts[b + 1] < T ? a.starts[b + 1] : T;
+  q.falls = e < s;
   if (e <= s) return q;
   q.start = s, q.past = a.past[b];
   q.rows = (int)(e - s) * REP;
@@ -233,12 +238,15 @@ __device__ __forceinline__ int many_splits(int kt, int part) {
 // split into parts of `part` key tiles each.
 struct Plan {
   int run, part, items, stride;    // items: of the many-row requests; stride: rows of a few-row partial
+  bool none;                       // starts fall: requests overlap, and may be more than the grid has room for
 };
 __device__ __forceinline__ Plan make_plan(const Args& a, Req& q) {
   const int lane = threadIdx.x & 63;
   float ud = 0, umax = 0, rmax = 0, up = 0, tp = 0;
+  bool falls = false;
   for (int b0 = 0; b0 < B; b0 += 64) {
     q = request(a, b0 + lane);
+    falls |= q.falls;
     if (q.tiles == 0) {
       ud += q.kt;
       umax = __builtin_fmaxf(umax, q.kt), rmax = __builtin_fmaxf(rmax, q.rows);
@@ -248,6 +256,7 @@ __device__ __forceinline__ Plan make_plan(const Args& a, Req& q) {
   }
   ud = sanic_wave_sum(ud), umax = sanic_wave_max(umax), rmax = sanic_wave_max(rmax);
   Plan p;
+  p.none = __any(falls);
   // whole 128-byte lines of statistics and sums: the workgroup that adds one request's parts reads no line
   // that holds another's, which its CU's L1 would keep as it was and a later join there would read
   p.stride = (__builtin_amdgcn_readfirstlane((int)rmax) + LINE - 1) / LINE * LINE;
@@ -906,6 +915,8 @@ extern "C" __global__ void __launch_bounds__(256, OCC) sanic_paged_attn(Args a) 
   int w = (int)(blockIdx.x / NKV);
   Req q;
   const Plan p = make_plan(a, q);
+  // (a run outside the grid would leave its request's arrivals part-counted, for later launches to find)
+  if (p.none) return;
   Item it;
   // the many-row items first: they take longest
   if (PITEMS && w < p.items) {

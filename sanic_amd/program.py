@@ -184,7 +184,8 @@ class Program:
         [NB, NKV, BS, HD], which hold the step's own rows too: request b's row i stands at
         past[b] + i and sees the keys up to there, with `window` > 0 the last `window` of them. Query
         head h reads key head h // (NH // NKV). A row that sees no key is 0; rows behind the last
-        request are left as they were. `scale` defaults to 1/√HD."""
+        request are left as they were, and so are all rows where `starts` falls. `scale` defaults to
+        1/√HD."""
         q, kc, vc, tables, starts, past = (self._operand(x) for x in (q, k_cache, v_cache, tables, starts, past))
         out = self._decl(name, role, q.shape, out_dtype)
         scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale

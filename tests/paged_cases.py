@@ -131,3 +131,13 @@ LOST_BLOCKS = {
     "blocks_of_one": dict(table=[[NONE, NONE - 1], [5, 6]], free=[NONE - 1, NONE, 2], past=[2, 2], new=[1, 2], block=1),
     "odd_block": dict(table=[[0xFFFFFFFF // 24], [0xFFFFFFFF // 24 + 1]], free=[5], past=[10, 3], new=[9, 9], block=24),
 }
+
+
+def falling_starts(HD, dq=ir.BF16):
+    """A batch of 64 rows, and starts that fall: 60 requests that claim all rows each, and single tokens
+    over long caches among them. (Σ rows is 60 times what the batch holds.)"""
+    past, new = [600] * 120 + [4000] * 64, [0] * 120 + [1] * 64
+    t = Batch(past=past, new=new, NKV=8, rep=4, HD=HD, BS=64, dq=dq)
+    starts = [0, 64] * 60 + list(range(65))
+    assert len(starts) == t.B + 1
+    return t, starts

@@ -10,7 +10,7 @@ import pytest
 
 import paged_ref as ref
 import wave_host as host
-from paged_cases import LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, LostBlocks, OddKey, OddQuery, OddValue
+from paged_cases import LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, LostBlocks, OddKey, OddQuery, OddValue, falling_starts
 from sanic_amd import ir
 from sanic_amd.backend import decode, encode
 from sanic_amd.program import NONE
@@ -140,6 +140,14 @@ def test_what_the_host_run_notices(folder, tmp_path):
             return text.replace(old, new)
         with pytest.raises(AssertionError, match=said):
             t.check(*attention(t, folder, tmp_path, change=change))
+
+
+@pytest.mark.parametrize("HD,dq", [(64, ir.BF16), (128, ir.F16), (24, ir.F32)])
+def test_starts_that_fall_leave_nothing_behind(HD, dq, folder, tmp_path):
+    """Overlapping requests can be more work than the launch has workgroups: nothing is begun."""
+    t, starts = falling_starts(HD, dq)
+    t.starts = np.zeros(t.B + 1, np.int64)      # every row is to be left as it was
+    attention(t, folder, tmp_path, starts, math=False)
 
 
 def _odd_value(case, folder, run_in):

@@ -1,8 +1,10 @@
 """The operators where values, indices or lengths are at the edge of what they may be, on the GPU: the
 cases of tests/test_cpu_operator_kernels.py again."""
+import numpy as np
 import pytest
 
-from paged_cases import LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, LostBlocks, OddKey, OddQuery, OddValue
+from paged_cases import LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, LostBlocks, OddKey, OddQuery, OddValue, falling_starts
+from sanic_amd import ir
 from test_gpu_operators import bind, read, words
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +43,20 @@ def test_lost_blocks_have_no_slots(dev, case):
     bufs = bind(dev, p, t.values())
     dev.prepare(p).execute_static(bufs)
     assert words(p, bufs, "plan.slots").tolist() == t.slots()
+
+
+@pytest.mark.parametrize("HD,dq", [(64, ir.BF16), (128, ir.F16), (24, ir.F32)])
+def test_starts_that_fall_leave_nothing_behind(dev, HD, dq):
+    """Nothing is written, and the next call (its arrivals are counted in the same words) is right."""
+    t, starts = falling_starts(HD, dq)
+    p = t.program()
+    bufs = bind(dev, p, t.values())
+    exe = dev.prepare(p)
+    for _ in range(2):
+        bufs["starts"].upload_array(np.asarray(starts, np.uint32))
+        bufs["o"].upload(b"\xa5" * p.by_name["o"].nbytes)
+        exe.execute_static(bufs)
+        assert bufs["o"].download() == b"\xa5" * p.by_name["o"].nbytes
+        bufs["starts"].upload_array(np.asarray(t.starts, np.uint32))
+        exe.execute_static(bufs)
+        t.check(read(p, bufs, "o"), exe.stage_kernel(0))

@@ -212,8 +212,13 @@ enum { SANIC_STAGE_FUSED = 0, SANIC_STAGE_POINTWISE = 1, SANIC_STAGE_OPERATOR = 
  *               past [B], scale (CONST); output [T, NH, HD]; stream = window, 0 = none. Query head h
  *               reads key head h / (NH / NKV). A row at position p sees the keys of positions
  *               j <= p, with a window j > p - window; keys without a block are not seen. Softmax of
- *               scale·q·k over them, in f32, times the values; a row that sees nothing is 0. A value
- *               that is not finite reaches every row that sees its key, however small the key's weight.
+ *               scale·q·k over them, in f32, times the values; a row that sees nothing, or scores of
+ *               -inf alone, is 0. A value that is not finite reaches every row that sees its key,
+ *               however small the key's weight. With 16-bit q and caches the weights go to the matrix
+ *               cores in the caches' type: with an f32 output as terms that hold 22 bits or more; with
+ *               a 16-bit output as two terms (16 bits of bf16, 22 of f16) for requests of up to 32
+ *               rows times NH / NKV, and rounded once, as the output is, for requests of more (RMS
+ *               error against 64 bits in bf16 2.3e-3, the output's rounding alone 1.7e-3).
  * VERIFY_DRAFTS leaves p [T, V], q [T, V] (or -1), tokens [T], u [T], draw [B], starts [B + 1],
  *               accepted [B]; output tokens [T]. tokens[r + 1] is the draft behind row r of the same
  *               request; p[r] are the target's probabilities there, q[r] those it was drawn from (no

@@ -1026,8 +1026,11 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     c += number("PAGES", 512) + number("FLIP", scale < 0) + "constexpr float C2 = " + flit(std::fabs(scale) * 1.4426950408889634) + ";\n";
     // Weights take the 16 bits of the matrix cores' operands. Few rows are bound by the cache's bytes: a
     // second term (what the rounding left) costs nothing there. Many rows are bound by the products and
-    // keep one term: half a step of relative error a weight, of both signs, in sums divided by the same
-    // rounded weights' sum. An f32 output gets 24 bits from three terms (f16: 22 from two, and the rest).
+    // keep one term where the output is 16 bits too: half a step of relative error a weight, of both signs,
+    // in sums divided by the same rounded weights' sum (RMS error against 64 bits, bf16, 2.3e-3; with two
+    // terms 1.7e-3, the output's own rounding, at 1499 us instead of 1186 for 4096 rows of heads of 128
+    // behind 12288 tokens, and 71.5 instead of 55.6 for a mixed batch of heads of 64). A caller that wants
+    // more asks for an f32 output: 24 bits from three terms (f16: 22 from two, and the rest; RMS 9e-8).
     c += number("FEW_TERMS", st.out_dtype == SANIC_F32 ? 3 : 2) + number("MANY_TERMS", st.out_dtype == SANIC_F32 ? 3 : 1);
     L.kernel_kind = "operator:paged_attn[mfma]";
     L.source = std::string(kPrelude) + kElement + c + kMfma;

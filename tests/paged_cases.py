@@ -141,3 +141,46 @@ def falling_starts(HD, dq=ir.BF16):
     starts = [0, 64] * 60 + list(range(65))
     assert len(starts) == t.B + 1
     return t, starts
+
+
+class Precision:
+    """How many bits of a softmax weight reach the output. Keys and queries are small whole numbers over
+    a power of two, so that every score is exact in 32 bits, at most 4.5, and what is left are the roundings
+    of score · log2 e (2^-24 of up to 6.5), of 2^x (the hardware's last place), and of the sums over at
+    most 90 keys: together below 2^-20 of an output's RMS for 24-bit weights. Weights of two bf16 terms
+    are rounded at 2^-17 (RMS 2^-19 to 2^-18 of an output), of one at 2^-9 (2^-10)."""
+
+    def __init__(self, new, dq, do, HD=64):
+        g = np.random.default_rng(new)
+        self.batch = t = Batch(past=[90 - new] * 3, new=[new] * 3, NKV=2, rep=4, HD=HD, BS=16, dq=dq, do=do, scale=2.0 ** -4)
+        t.q = g.integers(-1, 2, t.q.shape).astype(float)
+        t.kc = np.where(np.isnan(t.kc), np.nan, g.integers(-3, 4, t.kc.shape))
+        t.q[:, :, 24:] = 0.0          # |scores| <= 24 · 3 / 16 = 4.5
+
+    def rms(self, got):
+        o, _ = self.batch.want()
+        return float(np.sqrt(np.mean((got - o) ** 2) / np.mean(o ** 2)))
+
+    def steps(self, got):
+        """The error in units of half a step of the output's type at the exact value, the largest."""
+        o, mag = self.batch.want()
+        half = np.exp2(np.floor(np.log2(np.maximum(np.abs(o), 2.0 ** -14))) - (8 if self.batch.types[2] == ir.BF16 else 11))
+        return float((np.abs(got - o) / (half + 2.0 ** -15 * mag)).max())
+
+    def check(self, got, kind):
+        if self.batch.types[2] == ir.F32:
+            assert self.rms(got) < 2.0 ** -20, self.rms(got)
+        elif self.batch.new[0] * self.batch.rep <= 32:
+            # a few rows: 16 bits and more (2^-15 of the mean value, two times the weights' 2^-17 and as much
+            # again for the rest), then one rounding
+            assert self.steps(got) <= 1.0, self.steps(got)
+        else:
+            # many rows: one rounding of each weight to the cache's type, and the output's own; independent,
+            # at most half a step each, RMS half a step / √3 at worst
+            half = 2.0 ** -8 if self.batch.types[2] == ir.BF16 else 2.0 ** -11
+            assert self.rms(got) < half * np.sqrt(2.0 / 3.0), self.rms(got)
+
+
+PRECISION = {f"{'token' if n == 1 else 'drafts' if n < 9 else 'chunk'}_{x}_{y}": dict(new=n, dq=dq, do=do)
+             for n in (1, 8, 40) for x, dq, y, do in (("bf16", ir.BF16, "f32", ir.F32), ("f16", ir.F16, "f32", ir.F32), ("bf16", ir.BF16, "bf16", ir.BF16), ("f16", ir.F16, "f16", ir.F16))}
+HEADS = (16, 144, 176, 192, 208, 224, 240)

@@ -10,7 +10,7 @@ import pytest
 
 import paged_ref as ref
 import wave_host as host
-from paged_cases import LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, LostBlocks, OddKey, OddQuery, OddValue, falling_starts
+from paged_cases import HEADS, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, LostBlocks, OddKey, OddQuery, OddValue, Precision, falling_starts
 from sanic_amd import ir
 from sanic_amd.backend import decode, encode
 from sanic_amd.program import NONE
@@ -180,6 +180,36 @@ def _odd_query(case, folder, run_in):
 @run_alone(_odd_query)
 @pytest.mark.parametrize("case", ODD_QUERIES)
 def test_a_nan_in_a_query_is_in_its_row(case, results, request):
+    results[request.node.name].result()
+
+
+def _precision(case, folder, run_in):
+    """Passes, and would not with a term of the weights less."""
+    t = Precision(**PRECISION[case])
+    t.check(*attention(t.batch, folder, run_in))
+    name = "FEW_TERMS" if t.batch.new[0] * t.batch.rep <= 32 else "MANY_TERMS"
+    terms = host.constants(t.batch.program().emit(0)[1])[name]
+    if terms > 1 and t.batch.types[0] == ir.BF16:
+        less = lambda text: text.replace(f"constexpr int {name} = {terms};", f"constexpr int {name} = {terms - 1};")  # noqa: E731
+        with pytest.raises(AssertionError):
+            t.check(*attention(t.batch, folder, run_in, change=less))
+
+
+@run_alone(_precision)
+@pytest.mark.parametrize("case", PRECISION)
+def test_bits_of_the_weights(case, results, request):
+    results[request.node.name].result()
+
+
+def _heads(HD, folder, run_in):
+    for do in (ir.BF16, ir.F32):
+        t = Batch(past=[190, 99], new=[1, 30], NKV=1, rep=2, HD=HD, BS=16, do=do)
+        t.check(*attention(t, folder, run_in))
+
+
+@run_alone(_heads)
+@pytest.mark.parametrize("HD", HEADS)
+def test_every_head_size_on_the_cpu(HD, results, request):
     results[request.node.name].result()
 
 

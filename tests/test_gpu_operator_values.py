@@ -3,9 +3,9 @@ cases of tests/test_cpu_operator_kernels.py again."""
 import numpy as np
 import pytest
 
-from paged_cases import LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, LostBlocks, OddKey, OddQuery, OddValue, falling_starts
+from paged_cases import HEADS, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, LostBlocks, OddKey, OddQuery, OddValue, Precision, falling_starts
 from sanic_amd import ir
-from test_gpu_operators import bind, read, words
+from test_gpu_operators import Batch, bind, read, words
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +60,16 @@ def test_starts_that_fall_leave_nothing_behind(dev, HD, dq):
         bufs["starts"].upload_array(np.asarray(t.starts, np.uint32))
         exe.execute_static(bufs)
         t.check(read(p, bufs, "o"), exe.stage_kernel(0))
+
+
+@pytest.mark.parametrize("case", PRECISION)
+def test_bits_of_the_weights(dev, case):
+    t = Precision(**PRECISION[case])
+    t.check(*attention(dev, t.batch))
+
+
+@pytest.mark.parametrize("HD", HEADS)
+def test_every_head_size(dev, HD):
+    for do in (ir.BF16, ir.F32):
+        t = Batch(past=[190, 99], new=[1, 30], NKV=1, rep=2, HD=HD, BS=16, do=do)
+        t.check(*attention(dev, t))

@@ -1005,9 +1005,16 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     const int64_t PSPLIT = tiles ? std::min(2 * slots / NKV, budget / PR) : 0;
     const int64_t SLOTS = DROWS + PSPLIT * PR, per_head = groups + std::max(tiles, PSPLIT);
     // a workgroup's first key tile, its number times the run's length, stays within 31 bits
-    const int64_t most = M * BS / FEW_TK + 2, room = std::max<int64_t>(1, std::min(groups, DROWS / (2 * DR)));
-    const double run = 1.002 * std::max((double)B * most / room, (double)most / MOST) + 2;
-    if (!mfma_takes(q, k, v, B, M) || !std::isfinite(scale) || (per_head + 1) * run >= 2147483648.0) {
+    const int64_t most = M * BS / FEW_TK + 2, fit = std::max<int64_t>(1, std::min(groups, DROWS / (2 * DR)));
+    const double run = 1.002 * std::max((double)B * most / fit, (double)most / MOST) + 2;
+    // arrival counters: a head's on lines of their own (a line that several XCDs count on goes back and
+    // forth between them), each on one while the 16384 static ones last
+    int64_t cpad = 32;
+    auto counts = [&] { return ((B + PSPLIT / 2 + 1) * cpad + 31) / 32 * 32; };
+    while (cpad > 1 && counts() * NKV > 16384) cpad /= 2;
+    // two parts a key head of very many key heads, or their counters, would pass the static scratch
+    const bool room = NKV * (SLOTS * (HD + 2) + counts()) * 4 <= int64_t(28) << 20;
+    if (!mfma_takes(q, k, v, B, M) || !std::isfinite(scale) || (per_head + 1) * run >= 2147483648.0 || !room) {
         L.kernel_kind = "operator:paged_attn[plain]";
         L.source = std::string(kPrelude) + kElement + c + kPlain;
         L.launches.push_back(ln);
@@ -1016,11 +1023,6 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     c += number("FEW_TK", FEW_TK) + number("FEW_ST", FEW_ST) + number("MANY_TK", MANY_TK) + number("MANY_ST", MANY_ST);
     c += number("OCC", OCC) + number("PR", PR) + number("DR", DR) + number("MOST", MOST) + number("LINE", LINE);
     c += number("FEW_GROUPS", groups) + number("DROWS", DROWS) + number("PITEMS", tiles > 0) + number("PSPLIT", PSPLIT) + number("SLOTS", SLOTS);
-    // arrival counters: a head's on lines of their own (a line that several XCDs count on goes back and
-    // forth between them), each on one while the 16384 static ones last
-    int64_t cpad = 32;
-    auto counts = [&] { return ((B + PSPLIT / 2 + 1) * cpad + 31) / 32 * 32; };
-    while (cpad > 1 && counts() * NKV > 16384) cpad /= 2;
     c += number("COUNTS", counts()) + number("CPAD", cpad);
     c += number("ONE_XCD", xcd_local_enabled() && NKV % 8 == 0);
     c += number("PAGES", 512) + number("FLIP", scale < 0) + "constexpr float C2 = " + flit(std::fabs(scale) * 1.4426950408889634) + ";\n";

@@ -187,3 +187,9 @@ def test_programs_without_operators_say_so():
     p = configs.direct_attention()
     desc, keep = p.pack()
     assert int(keep[4][0]["op"]) == 0
+
+
+@pytest.mark.parametrize("NKV,T,kind", [(8, 5, "mfma"), (1024, 5, "mfma"), (1024, 40, "plain"), (4096, 1, "plain")])
+def test_many_key_heads_keep_to_the_static_scratch(NKV, T, kind):
+    """Where two parts a key head would not fit the partials' room, the kernel without parts takes the call."""
+    assert attn(NH=NKV, NKV=NKV, HD=128, T=T).emit(0)[0] == f"operator:paged_attn[{kind}]"

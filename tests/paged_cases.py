@@ -136,7 +136,7 @@ LOST_BLOCKS = {
 def falling_starts(HD, dq=ir.BF16):
     """A batch of 64 rows, and starts that fall: 60 requests that claim all rows each, and single tokens
     over long caches among them. (Σ rows is 60 times what the batch holds.)"""
-    past, new = [600] * 120 + [4000] * 64, [0] * 120 + [1] * 64
+    past, new = [100] * 120 + [900] * 64, [0] * 120 + [1] * 64
     t = Batch(past=past, new=new, NKV=8, rep=4, HD=HD, BS=64, dq=dq)
     starts = [0, 64] * 60 + list(range(65))
     assert len(starts) == t.B + 1
@@ -184,3 +184,22 @@ class Precision:
 PRECISION = {f"{'token' if n == 1 else 'drafts' if n < 9 else 'chunk'}_{x}_{y}": dict(new=n, dq=dq, do=do)
              for n in (1, 8, 40) for x, dq, y, do in (("bf16", ir.BF16, "f32", ir.F32), ("f16", ir.F16, "f32", ir.F32), ("bf16", ir.BF16, "bf16", ir.BF16), ("f16", ir.F16, "f16", ir.F16))}
 HEADS = (16, 144, 176, 192, 208, 224, 240)
+
+
+class SmallRoom(Batch):
+    """A batch in a program whose intermediates leave the attention the smaller area for its partials:
+    fewer runs of keys, and many rows that are not split or into few parts."""
+
+    def program(self, **kw):
+        p = super().program(**kw)
+        x = p.pointwise("ballast", ir.map_(ir.ADD, p.input("ballast.in", (26 << 18,), ir.F32), ir.const(1.0)), ir.F32, role=3)
+        p.pointwise("ballast.out", ir.map_(ir.ADD, x, ir.const(1.0)), ir.F32)
+        return p
+
+
+SMALL_ROOM = {
+    "decodes": dict(past=[300 * i % 1700 for i in range(70)], new=[1] * 70, NKV=8, rep=4, HD=128, BS=16),
+    "drafts": dict(past=[400 * i % 2100 for i in range(20)], new=[5] * 20, NKV=8, rep=4, HD=64, BS=32, dq=ir.F16),
+    "mixed": dict(past=[900, 40, 9, 0, 77, 1500], new=[1, 90, 0, 33, 1, 8], NKV=8, rep=4, HD=128, BS=16, pad=9),
+    "chunk": dict(past=[1500], new=[30], NKV=8, rep=4, HD=64, BS=16),
+}

@@ -10,7 +10,7 @@ import pytest
 
 import paged_ref as ref
 import wave_host as host
-from paged_cases import HEADS, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, LostBlocks, OddKey, OddQuery, OddValue, Precision, falling_starts
+from paged_cases import HEADS, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, SMALL_ROOM, LostBlocks, OddKey, OddQuery, OddValue, Precision, SmallRoom, falling_starts
 from sanic_amd import ir
 from sanic_amd.backend import decode, encode
 from sanic_amd.program import NONE
@@ -210,6 +210,19 @@ def _heads(HD, folder, run_in):
 @run_alone(_heads)
 @pytest.mark.parametrize("HD", HEADS)
 def test_every_head_size_on_the_cpu(HD, results, request):
+    results[request.node.name].result()
+
+
+def _small_room(case, folder, run_in):
+    t = SmallRoom(**SMALL_ROOM[case])
+    roomy, tight = (host.constants(p.emit(0)[1]) for p in (Batch.program(t), t.program()))
+    assert tight["SLOTS"] * 4 < roomy["SLOTS"]
+    t.check(*attention(t, folder, run_in))
+
+
+@run_alone(_small_room)
+@pytest.mark.parametrize("case", SMALL_ROOM)
+def test_little_room_for_partials(case, results, request):
     results[request.node.name].result()
 
 

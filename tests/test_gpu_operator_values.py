@@ -3,7 +3,7 @@ cases of tests/test_cpu_operator_kernels.py again."""
 import numpy as np
 import pytest
 
-from paged_cases import HEADS, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, LostBlocks, OddKey, OddQuery, OddValue, Precision, falling_starts
+from paged_cases import HEADS, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, SMALL_ROOM, LostBlocks, OddKey, OddQuery, OddValue, Precision, SmallRoom, falling_starts
 from sanic_amd import ir
 from test_gpu_operators import Batch, bind, read, words
 
@@ -73,3 +73,14 @@ def test_every_head_size(dev, HD):
     for do in (ir.BF16, ir.F32):
         t = Batch(past=[190, 99], new=[1, 30], NKV=1, rep=2, HD=HD, BS=16, do=do)
         t.check(*attention(dev, t))
+
+
+@pytest.mark.parametrize("case", SMALL_ROOM)
+def test_little_room_for_partials(dev, case):
+    t = SmallRoom(**SMALL_ROOM[case])
+    p = t.program()
+    bufs = bind(dev, p, {**t.values(), "ballast.in": np.zeros(p.by_name["ballast.in"].shape)})
+    exe = dev.prepare(p)
+    for _ in range(2):
+        exe.execute_static(bufs)
+        t.check(read(p, bufs, "o"), exe.stage_kernel(0))

@@ -993,9 +993,12 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     // of 32 and 4 workgroups, 63.5 and 77.5 for 2 workgroups). Heads of 128: 2 workgroups, many rows in
     // tiles of 64 in a ring of 2 (those 4096 rows 1660 us at that time; tiles of 32 in a ring of 3
     // 1770). Few-row workgroups as many as are resident: 2/3 of them 63.9 us for the drafts, twice as
-    // many 68.7, against 55.8.
+    // many 68.7, against 55.8. Heads of 160 to 256: a decode batch of 64 over up to 4000 tokens, 24 requests
+    // of 5 drafts over up to 3000, and 2048 rows behind 4096 tokens, us with 1 and with 2 workgroups a CU:
+    // 160 275 and 168, 132 and 117, 703 and 351; 192 286 and 182, 143 and 134, 743 and 376; 256 355 and 259,
+    // 219 and 204, 880 and 483. Rings of 3 instead of 2 are the same within 2% for all of these.
     const int64_t FEW_TK = HD <= 64 ? 64 : 32, FEW_ST = HD <= 64 ? 3 : HD <= 128 ? 4 : 2;
-    const int64_t MANY_TK = HD <= 128 ? 64 : 32, MANY_ST = HD <= 64 ? 3 : 2, OCC = HD <= 64 ? 3 : HD <= 192 ? 2 : 1;
+    const int64_t MANY_TK = HD <= 128 ? 64 : 32, MANY_ST = HD <= 64 ? 3 : 2, OCC = HD <= 64 ? 3 : 2;
     const int64_t PR = 128, DR = 32, MOST = 256, LINE = 16;
     const int64_t slots = 256 * OCC;
     const int64_t live = std::min(B, T), groups = std::max<int64_t>(1, slots / NKV);

@@ -233,7 +233,9 @@ LoweredStage lower_verify_drafts(const sanic_program_desc* d, const sanic_stage&
     else q = p;
     const int64_t T = p.extent[0], V = p.extent[1], B = d->nodes[st.leaf[4]].shape[0];
     // runs of 2048 entries, or so much longer that a batch has at most 4096 workgroups (two rounds of 8 a
-    // CU) and a request at most 1024
+    // CU) and a request at most 1024. With at most 512, 1024, 2048, 4096 and 8192: 64 requests of 128256
+    // entries with q 28.0, 24.3, 22.7, 23.5 and 23.4 us, 128 of them without q 36.4, 30.6, 28.4, 26.3 and
+    // 28.2, 200 of 32003 in bf16 22.0, 22.9, 20.2, 19.7 and 19.3
     int64_t turns = 1;
     auto runs = [&] { return (V + 2048 * turns - 1) / (2048 * turns); };
     while (runs() > 1 && (B * runs() > 4096 || runs() > 1024)) turns *= 2;

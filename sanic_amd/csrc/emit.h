@@ -82,6 +82,10 @@ int64_t shared_scratch(int64_t& scratch, int64_t bytes);
 int64_t shared_counters(int64_t n);
 // Bytes of the static scratch of sanic_hip_execute_static. A program whose first lowering needs more
 // is lowered again without the kernels that a form with less scratch can stand in for (lean).
+// The most that each of the two areas of partials of a paged attention may take: kPartialRoom, or less
+// where the program's other buffers leave less of the static scratch.
+const int64_t kPartialRoom = int64_t(12) << 20;
+int64_t partial_room();
 const int64_t kStaticScratchBytes = int64_t(32) << 20;
 bool lean_scratch();
 // Last-arriver handshake: the workgroups sharing counter `cnt` each add 1 once their partials

@@ -54,6 +54,8 @@ bool xcd_local_enabled() { return g_xcd_local.load(std::memory_order_relaxed) &&
 static thread_local int64_t t_counter_bytes = 0;
 static thread_local bool t_lean = false;
 bool lean_scratch() { return t_lean; }
+static thread_local int64_t t_partial_room = kPartialRoom;
+int64_t partial_room() { return t_partial_room; }
 int64_t take_counters(int64_t n) {
     const int64_t at = t_counter_bytes;
     t_counter_bytes += (n * 4 + 255) / 256 * 256;
@@ -1670,12 +1672,23 @@ Lowered lower_program(const sanic_program_desc* d) {
     auto fits = [&](const Lowered& l) { return l.scratch_bytes + 255 + l.counter_bytes + own <= kStaticScratchBytes; };
     Lowered out = lower_stages(d);
     if (fits(out)) return out;
-    struct Lean {
-        Lean() { t_lean = true; }
-        ~Lean() { t_lean = false; }
-    } lean;
-    Lowered less = lower_stages(d);
-    return fits(less) ? std::move(less) : std::move(out);
+    struct Less {
+        ~Less() { t_lean = false, t_partial_room = kPartialRoom; }
+    } restore;
+    // less room for the partials of a paged attention first, by a MiB at a time: its kernel is the same,
+    // with fewer runs of keys
+    bool partials = false;
+    for (int s = 0; s < d->n_stages; s++) partials = partials || (d->stages[s].kind == SANIC_STAGE_OPERATOR && d->stages[s].op == SANIC_OPR_PAGED_ATTN);
+    for (int lean = 0; lean < 2; lean++) {
+        t_lean = lean;
+        const int64_t mib = int64_t(1) << 20;
+        for (t_partial_room = partials ? kPartialRoom : mib; t_partial_room >= mib; t_partial_room -= mib) {
+            if (!lean && (!partials || t_partial_room == kPartialRoom)) continue;     // (that was the first)
+            Lowered less = lower_stages(d);
+            if (fits(less)) return less;
+        }
+    }
+    return out;
 }
 
 }  // namespace sanic

@@ -1002,7 +1002,7 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     const int64_t PR = 128, DR = 32, MOST = 256, LINE = 16;
     const int64_t slots = 256 * OCC;
     const int64_t live = std::min(B, T), groups = std::max<int64_t>(1, slots / NKV);
-    const int64_t budget = (lean_scratch() ? int64_t(1) << 20 : int64_t(12) << 20) / (NKV * (HD + 2) * 4);
+    const int64_t budget = partial_room() / (NKV * (HD + 2) * 4);
     const int64_t DROWS = std::min(2 * groups * std::min(DR, (T * REP + LINE - 1) / LINE * LINE), std::max(budget, 2 * DR)) / LINE * LINE;
     const int64_t tiles = T * REP > DR ? T * REP / PR + std::min(live, T * REP / (DR + 1)) : 0;
     const int64_t PSPLIT = tiles ? std::min(2 * slots / NKV, budget / PR) : 0;

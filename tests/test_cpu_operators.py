@@ -1,5 +1,7 @@
 """What the operators over ragged batches and paged caches refuse, on the CPU: shapes, types, roles
 and views, each before a kernel is compiled; and that what they accept lowers onto their kernels."""
+import re
+
 import pytest
 
 from sanic_amd import abi, configs, ir
@@ -193,3 +195,15 @@ def test_programs_without_operators_say_so():
 def test_many_key_heads_keep_to_the_static_scratch(NKV, T, kind):
     """Where two parts a key head would not fit the partials' room, the kernel without parts takes the call."""
     assert attn(NH=NKV, NKV=NKV, HD=128, T=T).emit(0)[0] == f"operator:paged_attn[{kind}]"
+
+
+@pytest.mark.parametrize("T,HD,runs", [(64, 128, 64), (1024, 128, 64), (1536, 128, 60), (2048, 128, 40), (1024, 64, 96), (2048, 64, 96)])
+def test_a_whole_step_keeps_its_runs_of_keys(T, HD, runs):
+    """The rotated rows of a long step take part of the static scratch: the attention's partials get what
+    is left of it, not a fixed small part. Runs a key head of requests of up to 16 packed rows."""
+    p = configs.paged_step(T, 41, 32, 8, HD, 4096, 16, 512)
+    i = next(i for i, st in enumerate(p.stages) if st.kind == 2 and st.op == 3)
+    kind, source = p.emit(i)
+    assert kind == "operator:paged_attn[mfma]"
+    c = {m[1]: int(m[2]) for m in re.finditer(r"constexpr int (\w+) = (\d+);", source)}
+    assert min(c["FEW_GROUPS"], c["DROWS"] // 32) >= runs

@@ -447,8 +447,9 @@ __device__ __forceinline__ float decay(float x) { return __builtin_fmaxf(__built
 
 // One column of scores into weights: s holds the products of the tile's keys row0 + 16·kt + r, of which
 // the row sees those in [lo, hi) that are no holes, and leaves as 2^(t − m). `factor` is what the row's earlier sums are scaled by.
+// A tile's maximum may exceed the reference by `lead`.
 template <int N>
-__device__ __forceinline__ void weigh(f32x4 (&s)[N], bool full, unsigned long long holes, int row0, int lo, int hi, float& m, float& factor) {
+__device__ __forceinline__ void weigh(f32x4 (&s)[N], bool full, unsigned long long holes, int row0, int lo, int hi, float lead, float& m, float& factor) {
   float top = NEG_INF;
   if (full) {
     #pragma unroll
@@ -466,9 +467,9 @@ __device__ __forceinline__ void weigh(f32x4 (&s)[N], bool full, unsigned long lo
       }
   }
   factor = 1.0f;
-  if (!__all(top <= m + 8.0f && m > NEG_INF)) {
+  if (!__all(top <= m + lead && m > NEG_INF)) {
     top = quad_max(top);
-    const float to = top > m + 8.0f ? top : m;
+    const float to = top > m + lead ? top : m;
     factor = to == m ? 1.0f : decay(m - to);
     m = to;
   }
@@ -494,7 +495,8 @@ __device__ __forceinline__ void weigh(f32x4 (&s)[N], bool full, unsigned long lo
 // adds it to the rows that see it. Tiles that every row sees whole are not cleaned: there a value that
 // is not finite goes through the product, which may make NaN of an infinite one (by a weight that is 0
 // in 32 bits, by the negative rest of a weight's first term). Rows whose sums come out not finite are
-// computed again with every tile cleaned. Rows [row0, row0 + rows) × chunks [c0, c0 + chunks), of which any row
+// computed again with every tile cleaned, and with the largest score so far as the reference (a lead of
+// 2^8 could take sums of values near the end of the range past it). Rows [row0, row0 + rows) × chunks [c0, c0 + chunks), of which any row
 // sees [lo, hi) (rows counted from the tile's first key).
 __device__ __forceinline__ unsigned long long clean(int tile, unsigned long long holes, int row0, int rows, int c0, int chunks, int lo, int hi, int part, int parts) {
   unsigned long long odd = 0;
@@ -684,7 +686,7 @@ __device__ __forceinline__ bool few_rows(const Args& a, const Item& it, int stri
       #pragma unroll
       for (int d = 0; d < DSTEP; d++) s[0] = mma32(key_run(Few::at(buf, 0), kg, d, l16, lq), qf[t][d], s[0]);
       float factor;
-      weigh<1>(s, full, holes, kg * 16 + lq * 4, lo[t] - t0, hi[t] - t0, m[t], factor);
+      weigh<1>(s, full, holes, kg * 16 + lq * 4, lo[t] - t0, hi[t] - t0, careful ? 0.0f : 8.0f, m[t], factor);
       if (!__all(factor == 1.0f)) {
         sum[t] *= factor;
         #pragma unroll
@@ -839,7 +841,7 @@ __device__ __forceinline__ bool many_rows(const Args& a, const Item& it, int g, 
       #pragma unroll
       for (int t = 0; t < 2; t++) {
         float factor;
-        weigh<NK>(s[t], full, holes, lq * 4, lo[t] - t0, hi[t] - t0, m[t], factor);
+        weigh<NK>(s[t], full, holes, lq * 4, lo[t] - t0, hi[t] - t0, careful ? 0.0f : 8.0f, m[t], factor);
         if (!__all(factor == 1.0f)) {
           sum[t] *= factor;
           #pragma unroll

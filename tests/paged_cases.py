@@ -203,3 +203,18 @@ SMALL_ROOM = {
     "mixed": dict(past=[900, 40, 9, 0, 77, 1500], new=[1, 90, 0, 33, 1, 8], NKV=8, rep=4, HD=128, BS=16, pad=9),
     "chunk": dict(past=[1500], new=[30], NKV=8, rep=4, HD=64, BS=16),
 }
+
+
+def huge_values(new, HD=64, requests=60):
+    """bf16 values of 10^36 under scores that rise by 5 behind the first keys: the weights' sums, relative to
+    the largest score, times the values stay within 32 bits' range (136 · 10^36), and so do the rows. So
+    many requests that a workgroup goes over several tiles of keys."""
+    t = Batch(past=[200] * requests, new=[new] * requests, NKV=8, rep=4, HD=HD, BS=16, scale=1.0)
+    t.q[:] = 0.0
+    t.q[:, :, 0] = 1.0
+    j = np.arange(200 + new)
+    for line in t.tables:
+        at = (line[j // 16].astype(int), slice(None), j % 16)
+        t.kc[at + (0,)] = np.where(j >= 64, 5.0, 0.0)[:, None]
+        t.vc[at] = stored(1e36 * (1.0 + 0.1 * t.vc[at].clip(-3, 3)), ir.BF16)
+    return t

@@ -10,7 +10,7 @@ import pytest
 
 import paged_ref as ref
 import wave_host as host
-from paged_cases import HEADS, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, SMALL_ROOM, LostBlocks, OddKey, OddQuery, OddValue, Precision, SmallRoom, falling_starts
+from paged_cases import HEADS, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, SMALL_ROOM, LostBlocks, OddKey, OddQuery, OddValue, Precision, SmallRoom, falling_starts, huge_values
 from sanic_amd import ir
 from sanic_amd.backend import decode, encode
 from sanic_amd.program import NONE
@@ -148,6 +148,17 @@ def test_starts_that_fall_leave_nothing_behind(HD, dq, folder, tmp_path):
     t, starts = falling_starts(HD, dq)
     t.starts = np.zeros(t.B + 1, np.int64)      # every row is to be left as it was
     attention(t, folder, tmp_path, starts, math=False)
+
+
+def _end_of_the_range(new, HD, folder, run_in):
+    t = huge_values(new, HD)
+    t.check(*attention(t, folder, run_in))
+
+
+@run_alone(_end_of_the_range)
+@pytest.mark.parametrize("new,HD", [(1, 64), (5, 128), (12, 64)])
+def test_values_near_the_end_of_the_range(new, HD, results, request):
+    results[request.node.name].result()
 
 
 def _odd_value(case, folder, run_in):

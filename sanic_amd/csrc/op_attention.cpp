@@ -62,12 +62,10 @@ extern "C" __global__ void __launch_bounds__(256) sanic_paged_attn(Args a) {
     const float top = __builtin_fmaxf(m, sanic_wave_max(s));
     // nothing seen so far, or only scores of -inf (whose weights are 0): no reference to subtract
     const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
-    // (above 0, so that an infinite value among the earlier ones stays one: next to the weight of 1 that
-    // moved the reference, 2^-126 is nothing)
-    const float w = seen ? __expf(s - ref) : 0.0f, c = __builtin_fmaxf(__expf(m - ref), 0x1p-126f);
+    const float w = seen ? __expf(s - ref) : 0.0f, c = __expf(m - ref);
     m = top;
     sum = sum * c + sanic_wave_sum(w);
-    for (int i = 0; i < DV; i++) o[i] *= c;
+    for (int i = 0; i < DV; i++) o[i] = __builtin_fabsf(o[i]) == __builtin_huge_valf() ? o[i] : o[i] * c;   // (a factor of 0 leaves it infinite)
     w_of[wave][lane] = w;
     page_of[wave][lane] = page;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -75,9 +73,13 @@ extern "C" __global__ void __launch_bounds__(256) sanic_paged_attn(Args a) {
       const unsigned pg = page_of[wave][x];
       if (pg >= NB) continue;   // a masked place's value may be anything, NaN among it
       const kv_t* v = a.v + (VB + pg * V0 + g * V1 + (base + x) % BS * V2);
-      const float wx = __builtin_fmaxf(w_of[wave][x], 0x1p-126f);   // a weight that is 0 in 32 bits is none of a seen key
+      const float wx = w_of[wave][x];
       for (int i = 0; i < DV; i++)
-        if (lane + 64 * i < HD) o[i] = __builtin_fmaf(wx, sanic_get<DC>(v[(lane + 64 * i) * V3]), o[i]);
+        if (lane + 64 * i < HD) {
+          // (a value that is not finite stays what it is, also at a weight that is 0 in 32 bits)
+          const float y = sanic_get<DC>(v[(lane + 64 * i) * V3]);
+          o[i] = __builtin_fabsf(y) < __builtin_huge_valf() ? __builtin_fmaf(wx, y, o[i]) : o[i] + y;
+        }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -441,9 +443,12 @@ __device__ __forceinline__ void tr_read8(unsigned even, s16x4 (&r)[8]) {
 }
 __device__ __forceinline__ bool odd_value(unsigned short x) { return HALF ? (x & 0x7C00) == 0x7C00 : (x & 0x7F80) == 0x7F80; }
 
-// What earlier sums are scaled by when the reference moves by -x: 2^x, but never 0, which would make NaN of
-// an infinite sum (next to the weight of 1 or more that moved the reference, 2^-126 is nothing).
-__device__ __forceinline__ float decay(float x) { return __builtin_fmaxf(__builtin_amdgcn_exp2f(x), 0x1p-126f); }
+// Sums scaled to another reference: an infinite one stays infinite where the factor is 0 in 32 bits.
+__device__ __forceinline__ f32x4 scaled(f32x4 v, float f) {
+  #pragma unroll
+  for (int r = 0; r < 4; r++) v[r] = __builtin_fabsf(v[r]) == __builtin_huge_valf() ? v[r] : v[r] * f;
+  return v;
+}
 
 // One column of scores into weights: s holds the products of the tile's keys row0 + 16·kt + r, of which
 // the row sees those in [lo, hi) that are no holes, and leaves as 2^(t − m). `factor` is what the row's earlier sums are scaled by.
@@ -470,7 +475,8 @@ __device__ __forceinline__ void weigh(f32x4 (&s)[N], bool full, unsigned long lo
   if (!__all(top <= m + lead && m > NEG_INF)) {
     top = quad_max(top);
     const float to = top > m + lead ? top : m;
-    factor = to == m ? 1.0f : decay(m - to);
+    // (without a reference so far there are no sums but 0 and what is not finite)
+    factor = to == m || m == NEG_INF ? 1.0f : __builtin_amdgcn_exp2f(m - to);
     m = to;
   }
   // nothing seen so far, or scores of −inf alone: their weights are 0, 2^(−inf − 0)
@@ -593,18 +599,27 @@ __device__ __forceinline__ void meet(const Args& a, const Item& it, int g, int r
     const int r = u / (HD / 4), d = u % (HD / 4) * 4;
     f32x4 acc = {0, 0, 0, 0};
     float m = NEG_INF, l = 0.0f;
-    auto add = [&](float m2, float l2, f32x4 v) {
+    auto add = [&](float m2, float l2, f32x4 v, bool careful) {
       const float to = __builtin_fmaxf(m, m2), ref = to == NEG_INF ? 0.0f : to;   // (a split that saw nothing has weight 0)
-      const float f = decay(m - ref), f2 = decay(m2 - ref);
-      acc = acc * f + v * f2;
+      const float f = __builtin_amdgcn_exp2f(m - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+      acc = careful ? scaled(acc, f) + scaled(v, f2) : acc * f + v * f2;
       l = l * f + l2 * f2;
       m = to;
     };
+    auto add_part = [&](int s, bool careful) {
+      const f32x2 x = *(const f32x2*)part_stats(a, g, place(s) + r);
+      add(x[0], x[1], *(const f32x4*)(part_sums(a, g, place(s) + r) + d), careful);
+    };
+    // where the sums are NaN, an infinite one may have met a factor of 0: they are added once more, with care
+    // (with care at once a single request's call takes 0.5 us of 11 more)
+    auto nan = [&] { const float x = (acc[0] + acc[1]) + (acc[2] + acc[3]); return x != x; };
     if (team < teams) {
       #pragma unroll 4
-      for (int s = team; s < splits; s += teams) {
-        const f32x2 x = *(const f32x2*)part_stats(a, g, place(s) + r);
-        add(x[0], x[1], *(const f32x4*)(part_sums(a, g, place(s) + r) + d));
+      for (int s = team; s < splits; s += teams) add_part(s, false);
+      if (nan()) {
+        acc = (f32x4){0, 0, 0, 0}, m = NEG_INF, l = 0.0f;
+        #pragma unroll 1
+        for (int s = team; s < splits; s += teams) add_part(s, true);
       }
     }
     if (teams > 1) {
@@ -614,7 +629,13 @@ __device__ __forceinline__ void meet(const Args& a, const Item& it, int g, int r
       stats[tid] = (f32x2){m, l};
       __syncthreads();
       if (team != 0) break;
-      for (int k = 1; k < teams; k++) add(stats[k * units + tid][0], stats[k * units + tid][1], sums[k * units + tid]);
+      auto add_team = [&](int k, bool careful) { add(stats[k * units + tid][0], stats[k * units + tid][1], sums[k * units + tid], careful); };
+      for (int k = 1; k < teams; k++) add_team(k, false);
+      if (nan()) {
+        acc = (f32x4){0, 0, 0, 0}, m = NEG_INF, l = 0.0f;
+        #pragma unroll 1
+        for (int k = 0; k < teams; k++) add_team(k, true);
+      }
     }
     put4(a.o + out_at(it, g, row0 + r) + d, l == 0.0f ? (f32x4){0, 0, 0, 0} : acc / l);
   }
@@ -690,7 +711,7 @@ __device__ __forceinline__ bool few_rows(const Args& a, const Item& it, int stri
       if (!__all(factor == 1.0f)) {
         sum[t] *= factor;
         #pragma unroll
-        for (int d = 0; d < DTH; d++) o[t][d] *= factor;
+        for (int d = 0; d < DTH; d++) o[t][d] = scaled(o[t][d], factor);
       }
       if (t == 0) few_values<0>(value_at(Few::at(buf, 1), l16, lq) + (kg * CG + (dt0 >> 1)) * 1024, vt);
       if (odd) add_odd<DTH>(st, odd, t0, lo[t] - t0, hi[t] - t0, o[t], dt0, lq);
@@ -723,10 +744,10 @@ __device__ __forceinline__ bool few_rows(const Args& a, const Item& it, int stri
     const int row = t * 16 + l16;
     float mx = NEG_INF;
     for (int k = 0; k < KG; k++) mx = __builtin_fmaxf(mx, stat[k * 32 + row]);
-    const float f = mx == NEG_INF ? 0.0f : decay(m[t] - mx);
+    const float f = mx == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m[t] - mx);
     #pragma unroll
     for (int d = 0; d < DTH; d++)
-      if (dt0 + d < DT) *(f32x4*)&acc[(kg * 16 * RT + row) * HD + (dt0 + d) * 16 + lq * 4] = o[t][d] * f;
+      if (dt0 + d < DT) *(f32x4*)&acc[(kg * 16 * RT + row) * HD + (dt0 + d) * 16 + lq * 4] = careful ? scaled(o[t][d], f) : o[t][d] * f;
   }
   __syncthreads();
   for (int u = tid; u < it.rows * (HD / 4); u += 256) {
@@ -845,7 +866,7 @@ __device__ __forceinline__ bool many_rows(const Args& a, const Item& it, int g, 
         if (!__all(factor == 1.0f)) {
           sum[t] *= factor;
           #pragma unroll
-          for (int d = 0; d < DT; d++) o[t][d] *= factor;
+          for (int d = 0; d < DT; d++) o[t][d] = scaled(o[t][d], factor);
         }
         if (odd) add_odd<DT>(st, odd, t0, lo[t] - t0, hi[t] - t0, o[t], 0, lq);
         #pragma unroll

@@ -218,3 +218,20 @@ def huge_values(new, HD=64, requests=60):
         t.kc[at + (0,)] = np.where(j >= 64, 5.0, 0.0)[:, None]
         t.vc[at] = stored(1e36 * (1.0 + 0.1 * t.vc[at].clip(-3, 3)), ir.BF16)
     return t
+
+
+def huge_far_values(new, HD=64, requests=1, dq=ir.BF16, value=2.0 ** 120):
+    """Values of 2^120 at the first keys, whose scores are so far below the others that their weights are
+    0 in 32 and in 64 bits: nothing of them is in any row."""
+    t = Batch(past=[200] * requests, new=[new] * requests, NKV=8, rep=4, HD=HD, BS=16, dq=dq)
+    t.q[:, :, 0] = 8.0
+    j = np.arange(70)
+    for line in t.tables:
+        at = (line[j // 16].astype(int), slice(None), j % 16)
+        t.kc[at + (0,)] = stored(-900.0 * HD ** 0.5, dq)
+        t.vc[at] = value
+    return t
+
+
+HUGE_FAR = {"token": dict(new=1), "token_128": dict(new=1, HD=128), "drafts": dict(new=5), "chunk": dict(new=40), "tokens_60": dict(new=1, requests=60),
+            "chunks_60": dict(new=12, requests=60), "head_24": dict(new=2, HD=24), "f32": dict(new=2, dq=ir.F32)}

@@ -10,7 +10,7 @@ import pytest
 
 import paged_ref as ref
 import wave_host as host
-from paged_cases import HEADS, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, SMALL_ROOM, LostBlocks, OddKey, OddQuery, OddValue, Precision, SmallRoom, falling_starts, huge_values
+from paged_cases import HEADS, HUGE_FAR, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, SMALL_ROOM, LostBlocks, OddKey, OddQuery, OddValue, Precision, SmallRoom, falling_starts, huge_far_values, huge_values
 from sanic_amd import ir
 from sanic_amd.backend import decode, encode
 from sanic_amd.program import NONE
@@ -158,6 +158,17 @@ def _end_of_the_range(new, HD, folder, run_in):
 @run_alone(_end_of_the_range)
 @pytest.mark.parametrize("new,HD", [(1, 64), (5, 128), (12, 64)])
 def test_values_near_the_end_of_the_range(new, HD, results, request):
+    results[request.node.name].result()
+
+
+def _huge_far(case, folder, run_in):
+    t = huge_far_values(**HUGE_FAR[case])
+    t.check(*attention(t, folder, run_in))
+
+
+@run_alone(_huge_far)
+@pytest.mark.parametrize("case", HUGE_FAR)
+def test_huge_values_without_weight(case, results, request):
     results[request.node.name].result()
 
 

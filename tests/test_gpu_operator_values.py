@@ -3,7 +3,7 @@ cases of tests/test_cpu_operator_kernels.py again."""
 import numpy as np
 import pytest
 
-from paged_cases import HEADS, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, SMALL_ROOM, LostBlocks, OddKey, OddQuery, OddValue, Precision, SmallRoom, falling_starts, huge_values
+from paged_cases import HEADS, HUGE_FAR, LOST_BLOCKS, ODD_KEYS, ODD_QUERIES, ODD_VALUES, PRECISION, SMALL_ROOM, LostBlocks, OddKey, OddQuery, OddValue, Precision, SmallRoom, falling_starts, huge_far_values, huge_values
 from sanic_amd import ir
 from test_gpu_operators import Batch, bind, read, words
 
@@ -89,4 +89,10 @@ def test_little_room_for_partials(dev, case):
 @pytest.mark.parametrize("new,HD", [(1, 64), (5, 128), (12, 64)])
 def test_values_near_the_end_of_the_range(dev, new, HD):
     t = huge_values(new, HD)
+    t.check(*attention(dev, t))
+
+
+@pytest.mark.parametrize("case", HUGE_FAR)
+def test_huge_values_without_weight(dev, case):
+    t = huge_far_values(**HUGE_FAR[case])
     t.check(*attention(dev, t))

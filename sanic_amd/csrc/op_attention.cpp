@@ -14,7 +14,7 @@ namespace sanic {
 // for the output; m, the sum and the output in f32 over one pass. For every type, head size and
 // layout. Bound by its f32 operations and by reading every key once a row: 16 to 70 times the
 // matrix-core kernel's time where both can run (a token of each of 64 requests 3848 us against 236, 4096
-// rows of a prompt behind 12288 tokens 82.9 ms against 1.16).
+// rows of a prompt behind 12288 tokens 82.9 ms against 1.19).
 static const char* kPlain = R"SRC(
 typedef sanic_elem<DQ>::T q_t;
 typedef sanic_elem<DC>::T kv_t;
@@ -101,18 +101,20 @@ extern "C" __global__ void __launch_bounds__(256) sanic_paged_attn(Args a) {
 // Work is split over keys too. Request lengths are known on the device alone, so every workgroup sums
 // the requests' key tiles and derives the same plan. The few-row requests' tiles, one request behind
 // the other, are cut into as many equal runs as workgroups are resident: a run may end one request and
-// begin the next, and no workgroup has more than another (24 requests of 5 drafts: 55 us; an item a
+// begin the next, and no workgroup has more than another (24 requests of 5 drafts: 55 us, now 50; an item a
 // workgroup, with the longest request's items last, 68). Many-row tiles are split into parts over the
 // keys. Either way the partials fit the scratch. The parts of one row meet in the workgroup that
 // arrives last, which adds them in split order. The arrivals are relaxed where a key head's workgroups
 // share an XCD, whose L2 they meet in (a release writes that L2 back: 103 us instead of 68).
 //
 // Bound by HBM for decoded tokens: 64 requests of 32/8 heads of 128, 1.2 GB of cache, 236 us, 5.1 TB/s
-// (a large copy: 5.2); 10 us for one request, a chain of dependent loads. Bound by the matrix cores for
-// a prompt: 4096 rows of 32/8 heads of 128 behind 12288 tokens, 1157 us, 831 TFLOP/s (a large product: 1235). What brought
+// (a large copy: 5.2); 10.8 us for one request, a chain of dependent loads. Bound by matrix and vector
+// instructions for a prompt (38% and 36% of the SIMDs' cycles): 4096 rows of 32/8 heads of 128 behind 12288
+// tokens, 1107 to 1187 us by the card, 811 to 869 TFLOP/s (a large product: 1235). What brought
 // it there from 2911 us: tiles as blocks of 1 KB whose reads differ by constant offsets, and eight
 // transposed reads to one wait (1795); page addresses in scalar registers (1157; the 64 requests 310 to
-// 236).
+// 236). Finding sums that are not finite, and what a second pass over such rows needs, took 0.5 us of a
+// single request's call and 2% of that prompt's.
 //
 // Scores are computed transposed (Sᵀ = K·Qᵀ), so a lane owns one row's column: softmax statistics are
 // lane-local plus two lane swaps, and Sᵀ's layout is the B operand of Oᵀ = Vᵀ·P as it stands. Softmax

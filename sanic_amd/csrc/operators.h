@@ -29,8 +29,8 @@ LoweredStage lower_verify_drafts(const sanic_program_desc* d, const sanic_stage&
 
 // "constexpr long long NAME = value;" for a generated source
 std::string constant(const char* name, int64_t v);
-// Kernel functions: load one element of a float type as f32, store f32 as one (LD<code>, ST<code> by
-// the dtype's template argument), and the type names the operators' sources use.
+// Kernel functions: one element of a float type as f32 (sanic_get<code>), f32 rounded to one
+// (sanic_put<code>), and the storage types by their code (sanic_elem<code>::T).
 extern const char* kElement;
 
 }  // namespace sanic

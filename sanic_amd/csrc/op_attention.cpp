@@ -1041,7 +1041,7 @@ LoweredStage lower_paged_attn(const sanic_program_desc* d, const sanic_stage& st
     auto counts = [&] { return ((B + PSPLIT / 2 + 1) * cpad + 31) / 32 * 32; };
     while (cpad > 1 && counts() * NKV > 16384) cpad /= 2;
     // two parts a key head of very many key heads, or their counters, would pass the static scratch
-    const bool room = NKV * (SLOTS * (HD + 2) + counts()) * 4 <= int64_t(28) << 20;
+    const bool room = NKV * (SLOTS * (HD + 2) + counts()) * 4 <= 2 * kPartialRoom + (int64_t(1) << 20);
     if (!mfma_takes(q, k, v, B, M) || !std::isfinite(scale) || (per_head + 1) * run >= 2147483648.0 || !room) {
         L.kernel_kind = "operator:paged_attn[plain]";
         L.source = std::string(kPrelude) + kElement + c + kPlain;
